@@ -401,6 +401,107 @@ tir_status tir_attention(const float *q, const float *k_cache, const float *v_ca
                          float *out, int64_t q_heads, int64_t k_v_heads, int64_t dim,
                          int64_t n_ctx, int64_t max_ctx, void *stream);
 
+/* ---- paged key-value cache (runtime extension; the reference keeps one
+ * unbounded f32 Cache per request, src/data.rs:41-51) -----------------------
+ * Operators between a step's q|k|v projection and its output projection, over
+ * a cache that the caller owns: pages of `page_size` positions in a pool, a
+ * page table on the device.  Activations are f32, f16 or bf16; a cache is f32,
+ * f16, bf16 or Q8_0 (blocks of 32 values, quantised by activated_q8's rule,
+ * src/kernels.rs:8-31, as they are written).  All run asynchronously on
+ * `stream` of the current device and can be captured into a graph after one
+ * earlier call on that device.  They allocate nothing.  What the host cannot
+ * check (a page id outside the pool, a position outside the table) is skipped
+ * by the kernels and reported by tir_ops_check as TIR_ERR_INVALID_ARG. */
+
+/* Element types beside TIR_DTYPE_F32 and TIR_DTYPE_Q8_0 (GGUF's codes). */
+enum { TIR_DTYPE_F16 = 1, TIR_DTYPE_BF16 = 30 };
+
+/* A paged cache in device memory.  Element (page, slot, head, c) of keys and
+ * values is at page * page_stride + slot * pos_stride + head * head_stride + c
+ * (strides in elements, one layout for both pools).  For Q8_0, `k` and `v`
+ * hold the int8 quants and k_scale / v_scale the f16 steps, that of the block
+ * at element offset e at index e / 32.  `table` holds, per sequence, the pages
+ * of its positions in order: position p is slot p % page_size of page
+ * table[row * table_stride + p / page_size].  dim is 64, 128 or 256; pools are
+ * 16-byte aligned, strides multiples of 16 bytes (Q8_0: of dim). */
+typedef struct tir_kv_pages {
+    void *k, *v;
+    uint16_t *k_scale, *v_scale;  /* Q8_0 only */
+    const int32_t *table;
+    int64_t table_rows, table_stride;
+    int64_t n_pages;
+    int64_t page_stride, pos_stride, head_stride;
+    int32_t max_pages;            /* table columns in use */
+    int32_t page_size;
+    int32_t kv_heads, dim;
+    int32_t dtype;                /* TIR_DTYPE_F32, _F16, _BF16 or _Q8_0 */
+} tir_kv_pages;
+
+/* Which elements of a head the rotation pairs: (2 i, 2 i + 1) as rope
+ * (src/math.rs:196-228), or (i, i + rope_dim / 2). */
+enum { TIR_PAIRS_ADJACENT = 0, TIR_PAIRS_HALVES = 1 };
+
+/* What happens to each query and key head: rmsnorm over the head (src/math.rs:
+ * 141-150 with this eps and weight; NULL weight: none), then the rotation of
+ * its first rope_dim elements (a multiple of 16; rope NULL: none) by the cos
+ * and sin in row `position` of a device table [rope_positions][rope_dim / 2][2]
+ * (tir_rope_table). */
+typedef struct tir_qk_norm {
+    const float *q_weight, *k_weight;
+    const float *rope;
+    int64_t rope_positions;
+    int32_t rope_dim;
+    int32_t pairs;
+    float eps;
+} tir_qk_norm;
+
+/* cos and sin of rope_angles (src/math.rs:181-193) for positions 0..n_pos-1,
+ * host: out_host [n_pos][dim / 2][2]. */
+tir_status tir_rope_table(float base, int64_t dim, int64_t n_pos, float *out_host);
+
+/* Norm and rotation in one pass: q_out, k_out from q [tokens][q_heads][dim]
+ * and k [tokens][kv_heads][dim], strides in elements between tokens (a token's
+ * heads are adjacent; q, k may be parts of one q|k|v row).  f32 inside, rounded
+ * once.  In place (q_out == q with the same stride) is allowed, any other
+ * overlap is not.  positions [tokens], NULL only without a rotation; a token
+ * whose position is negative is left out, its outputs as they were. */
+tir_status tir_qk_norm_rope(const void *q, int64_t q_stride, const void *k, int64_t k_stride, void *q_out,
+                            int64_t q_out_stride, void *k_out, int64_t k_out_stride, const int32_t *positions,
+                            int64_t tokens, int32_t q_heads, int32_t kv_heads, int32_t dim, int32_t dtype,
+                            const tir_qk_norm *norm, void *stream);
+/* The same with the keys, and the values as they are, written to the cache:
+ * token t to position positions[t] of table row seqs[t] (NULL: row t).  Two
+ * tokens of a call must not share a slot. */
+tir_status tir_qk_norm_rope_append(const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
+                                   int64_t v_stride, void *q_out, int64_t q_out_stride, const tir_kv_pages *kv,
+                                   const int32_t *seqs, const int32_t *positions, int64_t tokens, int32_t q_heads,
+                                   int32_t dtype, const tir_qk_norm *norm, void *stream);
+/* Rows k, v [tokens][kv_heads][dim] of `dtype` to the cache, rounded or
+ * quantised; slots as above. */
+tir_status tir_kv_append(const tir_kv_pages *kv, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                         const int32_t *seqs, const int32_t *positions, int64_t tokens, int32_t dtype, void *stream);
+/* Cached positions back as rows of `dtype`, in any order, repeats allowed; a
+ * row whose position is negative is left as it was. */
+tir_status tir_kv_gather(const tir_kv_pages *kv, void *k_out, int64_t k_out_stride, void *v_out, int64_t v_out_stride,
+                         const int32_t *seqs, const int32_t *positions, int64_t tokens, int32_t dtype, void *stream);
+
+/* Grouped-query attention (src/forward.rs:86-174) of one query token per
+ * sequence over its pages: row r of q [rows][q_heads][dim] over positions
+ * [max(0, seq_lens[r] - window), seq_lens[r]) of table row r (window 0: all).
+ * seq_lens is on the device and counts the token itself once it is appended; a
+ * row of length 0 gets zeros.  scale multiplies the scores (0: 1 / sqrt(dim)).
+ * out has q's type.  f32 queries go with any cache, 16-bit ones with a cache of
+ * their own type or Q8_0.  max_len, at least the longest length (0: what the
+ * table holds), only sizes the split of long rows over the GPU.  workspace:
+ * tir_paged_attention_workspace bytes (0: none is needed, -1: sizes that are
+ * refused), 16-byte aligned, of any content, not shared by calls that can run at the same time. */
+int64_t tir_paged_attention_workspace(const tir_kv_pages *kv, int64_t rows, int32_t q_heads, int64_t max_len,
+                                      int64_t window);
+tir_status tir_paged_attention(const void *q, int64_t q_stride, const tir_kv_pages *kv, const int32_t *seq_lens,
+                               void *out, int64_t out_stride, int64_t rows, int32_t q_heads, int32_t dtype,
+                               float scale, int64_t max_len, int64_t window, void *workspace,
+                               int64_t workspace_bytes, void *stream);
+
 /* The op entry points above run asynchronously on the caller's stream, so a
  * bounded device-side wait that gave up (TIR_TIMEOUT_MS) inside one of them
  * cannot be returned by the call itself.  tir_ops_check synchronises `stream`
@@ -409,8 +510,11 @@ tir_status tir_attention(const float *q, const float *k_cache, const float *v_ca
  * tir_q8_matmul_batch), clearing the record; TIR_OK otherwise.  No launch
  * starts with an earlier launch's failure in its error words (a matvec's
  * last CTA to exit clears them; the tensor-core op clears them before it
- * starts), so one failure does not make later calls skip their work.  Runtime extension; no counterpart in the
- * reference, whose ops are synchronous CPU code. */
+ * starts), so one failure does not make later calls skip their work.
+ * A paged-cache operator that met a bad page id, position or length on this
+ * device is reported once as TIR_ERR_INVALID_ARG (after a timeout, by the next
+ * check).  Runtime extension; no counterpart in the reference, whose ops are
+ * synchronous CPU code. */
 tir_status tir_ops_check(void *stream);
 
 /* ---- test hooks (runtime extensions; no counterpart in the reference) ----

@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "host.h"
+#include "paged.h"
 #include "runtime.h"
 
 #define TIR_VERSION "0.1.0-sm100a"
@@ -1343,6 +1344,15 @@ tir_status tir_ops_check(void* stream) {
     if (code != 0u || scode != 0u)
         return fail(TIR_ERR_TIMEOUT, "a device-side wait of an op launched on device " + std::to_string(dev) +
                                          " gave up (TIR_TIMEOUT_MS); its outputs are incomplete");
+    uint32_t bad = 0;
+    const tir_status prc = paged_take_error(dev, &bad);
+    if (prc != TIR_OK) return prc;
+    if (bad != 0u)
+        return fail(TIR_ERR_INVALID_ARG, "a paged cache operator on device " + std::to_string(dev) + " met" +
+                                             (bad & kBadPage ? " a page id outside the pool" : "") +
+                                             (bad & kBadPosition ? " a position or sequence outside its table" : "") +
+                                             (bad & kBadLength ? " a length its table cannot hold" : "") +
+                                             "; it skipped those accesses");
     return TIR_OK;
 }
 

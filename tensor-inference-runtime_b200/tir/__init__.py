@@ -52,6 +52,21 @@ class TensorInfo(C.Structure):
                 ("dtype", C.c_uint32), ("offset", C.c_uint64), ("data_bytes", C.c_uint64)]
 
 
+class KVPagesDesc(C.Structure):
+    """tir_kv_pages."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("table", C.c_void_p), ("table_rows", C.c_int64), ("table_stride", C.c_int64),
+                ("n_pages", C.c_int64), ("page_stride", C.c_int64), ("pos_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("max_pages", C.c_int32), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class QKNorm(C.Structure):
+    """tir_qk_norm."""
+    _fields_ = [("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("rope", C.c_void_p),
+                ("rope_positions", C.c_int64), ("rope_dim", C.c_int32), ("pairs", C.c_int32), ("eps", C.c_float)]
+
+
 class Transformer(C.Structure):
     _fields_ = [("layers", C.c_uint32), ("dim", C.c_uint64), ("embed_dim", C.c_uint64),
                 ("q_heads", C.c_uint64), ("k_v_heads", C.c_uint64), ("base_freq", C.c_float),
@@ -156,6 +171,16 @@ SIGNATURES = {
     "tir_q8_act_matmul": (C.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "tir_argmax": (C.c_int, [_vp, _i64, _vp, _vp]),
     "tir_attention": (C.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "tir_rope_table": (C.c_int, [C.c_float, _i64, _i64, _f32p]),
+    "tir_qk_norm_rope": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, C.c_int32, C.c_int32,
+                                   C.c_int32, C.c_int32, _vp, _vp]),
+    "tir_qk_norm_rope_append": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64,
+                                          C.c_int32, C.c_int32, _vp, _vp]),
+    "tir_kv_append": (C.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, C.c_int32, _vp]),
+    "tir_kv_gather": (C.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, C.c_int32, _vp]),
+    "tir_paged_attention_workspace": (_i64, [_vp, _i64, C.c_int32, _i64, _i64]),
+    "tir_paged_attention": (C.c_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, C.c_int32, C.c_int32, C.c_float, _i64,
+                                      _i64, _vp, _i64, _vp]),
     "tir_ops_check": (C.c_int, [_vp]),
     "tir_debug_fail_alloc_after": (None, [_i64]),
     "tir_debug_alloc_count": (_i64, []),
@@ -784,3 +809,245 @@ def argmax(x, n, out_id, stream=None):
 def attention(q, k_cache, v_cache, out, q_heads, k_v_heads, dim, n_ctx, max_ctx, stream=None):
     check(lib().tir_attention(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), q_heads, k_v_heads,
                               dim, n_ctx, max_ctx, _stream(stream)))
+
+
+# ---------------------------------------------------------------------------
+# paged key-value cache (CUDA torch tensors)
+# ---------------------------------------------------------------------------
+DTYPE_F32, DTYPE_F16, DTYPE_Q8_0, DTYPE_BF16 = 0, 1, 8, 30
+PAIRS = {"adjacent": 0, "halves": 1}
+
+
+def _bad(message):
+    return TirError(23, message)  # INVALID_ARG
+
+
+def _codes():
+    """torch dtype -> TIR_DTYPE_* of activations; filled on first use (torch is
+    imported only by callers that hold tensors)."""
+    if not _CODES:
+        import torch
+        _CODES.update({torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16})
+    return _CODES
+
+
+_CODES = {}
+
+
+def _rows(x, heads, dim, code, device, what):
+    """Checks a [tokens, heads, dim] tensor whose heads are adjacent; returns
+    (pointer, stride between tokens in elements, tokens)."""
+    shape = x.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise _bad(f"{what} must be [tokens, {heads}, {dim}], got {list(shape)}")
+    stride = x.stride()
+    if stride[2] != 1 or (stride[1] != dim and heads > 1):
+        raise _bad(f"{what}: a token's heads must be adjacent")
+    if _codes().get(x.dtype) != code:
+        raise _bad(f"{what} has another type than q or k: {x.dtype}")
+    if x.get_device() != device:
+        raise _bad(f"{what} is not on device {device}")
+    return x.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], heads * dim), shape[0]
+
+
+def _ints(x, n, device, what):
+    """Pointer of a contiguous int32 tensor of at least n values (None: NULL)."""
+    if x is None:
+        return None
+    if x.numel() < n or x.dim() != 1 or (n > 1 and x.stride(0) != 1) or x.element_size() != 4 or \
+            x.is_floating_point():
+        raise _bad(f"{what} must be a contiguous int32 vector of {n} values")
+    if x.get_device() != device:
+        raise _bad(f"{what} is not on device {device}")
+    return x.data_ptr()
+
+
+def _act(x, what):
+    code = _codes().get(x.dtype)
+    if code is None:
+        raise TirError(6, f"{what}: activations must be float32, float16 or bfloat16, got {x.dtype}")
+    return code
+
+
+def _here(device):
+    """The operators launch on the current device; their tensors must be there."""
+    if device < 0:
+        raise _bad("the cache and the activations must be on a CUDA device")
+    import torch
+    if device != torch.cuda.current_device():
+        raise _bad(f"the cache or activations are on device {device}, the current device is "
+                   f"{torch.cuda.current_device()}")
+
+
+class KVPages:
+    """A paged key-value cache (tir_kv_pages) over caller-owned tensors.
+
+    k, v: [n_pages, page_size, kv_heads, dim], float32, float16, bfloat16 or (with
+    k_scale, v_scale) int8 Q8_0 quants, dim contiguous, the other strides free but
+    equal in both (a permuted view of another order is fine).  k_scale, v_scale:
+    float16 [n_pages, page_size, kv_heads, dim / 32] in the same order.  table:
+    int32 [rows, max_pages] on the device; its content may change between calls."""
+
+    def __init__(self, k, v, table, k_scale=None, v_scale=None):
+        import torch
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+            raise _bad("k and v must be [n_pages, page_size, kv_heads, dim] of one shape, stride and type")
+        if k.stride(3) != 1:
+            raise _bad("a head's elements must be adjacent")
+        if k.dtype == torch.int8:
+            code = DTYPE_Q8_0
+            if k_scale is None or v_scale is None:
+                raise _bad("an int8 cache needs k_scale and v_scale")
+            for s in (k_scale, v_scale):
+                if s.dtype != torch.float16 or tuple(s.shape) != (*k.shape[:3], k.shape[3] // 32) or \
+                        s.stride(3) != 1 or any(32 * a != b for a, b, n in zip(s.stride()[:3], k.stride()[:3], k.shape)
+                                                if n > 1):
+                    raise _bad("scales must be float16 [n_pages, page_size, kv_heads, dim / 32] in the quants' order")
+        else:
+            code = _act(k, "k")
+            if k_scale is not None or v_scale is not None:
+                raise _bad("scales belong to an int8 cache")
+        if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise _bad("table must be int32 [rows, max_pages]")
+        self.device = k.get_device()
+        for x in (v, table, k_scale, v_scale):
+            if x is not None and x.get_device() != self.device:
+                raise _bad("the cache's tensors must be on one CUDA device")
+        if self.device < 0:
+            raise _bad("the cache's tensors must be on a CUDA device")
+        self.k, self.v, self.table, self.k_scale, self.v_scale = k, v, table, k_scale, v_scale
+        self.kv_heads, self.dim, self.page_size = int(k.shape[2]), int(k.shape[3]), int(k.shape[1])
+        rows, cols = table.shape
+        # the stride of a dimension of one entry is never used: give it one that fits
+        st = [s if n > 1 else self.dim for s, n in zip(k.stride()[:3], k.shape)]
+        self.desc = KVPagesDesc(k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), rows,
+                                table.stride(0) if rows > 1 else max(cols, 1), k.shape[0], st[0], st[1], st[2], cols,
+                                self.page_size, self.kv_heads, self.dim, code)
+        self.ref = C.addressof(self.desc)
+
+
+def rope_table(base, dim, n_pos):
+    """cos and sin of rope_angles for positions 0..n_pos-1: float32 [n_pos, dim / 2, 2]."""
+    out = np.empty((n_pos, dim // 2, 2), np.float32)
+    check(lib().tir_rope_table(float(base), dim, n_pos, out.ctypes.data_as(_f32p)))
+    return out
+
+
+def _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device):
+    import torch
+    if pairs not in PAIRS:
+        raise _bad(f"pairs must be one of {sorted(PAIRS)}")
+    n_pos = rope_dim = 0
+    if rope is not None:
+        if rope.dim() != 3 or rope.shape[2] != 2 or not rope.is_contiguous() or rope.dtype != torch.float32:
+            raise _bad("rope must be a contiguous float32 [positions, rope_dim / 2, 2] table")
+        n_pos, rope_dim = rope.shape[0], 2 * rope.shape[1]
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dim() != 1 or w.shape[0] != dim or w.dtype != torch.float32 or w.stride(0) != 1):
+            raise _bad(f"a norm weight must be a contiguous float32 vector of {dim}")
+    for x in (rope, q_weight, k_weight):
+        if x is not None and x.get_device() != device:
+            raise _bad(f"rotation table and weights must be on device {device}")
+    return QKNorm(_ptr(q_weight), _ptr(k_weight), _ptr(rope), n_pos, rope_dim, PAIRS[pairs], eps)
+
+
+def _tokens_of(*rows):
+    n = rows[0][2]
+    if any(r[2] != n for r in rows):
+        raise _bad("rows of different token counts")
+    return n
+
+
+def qk_norm_rope(q, k, q_out, k_out, positions, rope=None, q_weight=None, k_weight=None, eps=1e-5, pairs="adjacent",
+                 stream=None):
+    """Per-head rmsnorm (where a weight is given) and rotation of q [tokens,
+    q_heads, dim] and k [tokens, kv_heads, dim] into q_out and k_out (which may be
+    q and k).  positions int32 [tokens]; a negative one leaves its token out."""
+    code, device = _act(q, "q"), q.get_device()
+    _here(device)
+    if q.dim() != 3 or k.dim() != 3:
+        raise _bad("q and k must be [tokens, heads, dim]")
+    qh, kh, dim = q.shape[1], k.shape[1], q.shape[2]
+    a, b = _rows(q, qh, dim, code, device, "q"), _rows(k, kh, dim, code, device, "k")
+    c, d = _rows(q_out, qh, dim, code, device, "q_out"), _rows(k_out, kh, dim, code, device, "k_out")
+    n = _tokens_of(a, b, c, d)
+    norm = _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device)
+    check(lib().tir_qk_norm_rope(a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1],
+                                 _ints(positions, n, device, "positions"), n, qh, kh, dim, code, C.addressof(norm),
+                                 _stream(stream)))
+
+
+def qk_norm_rope_append(q, k, v, q_out, kv, seqs, positions, rope=None, q_weight=None, k_weight=None, eps=1e-5,
+                        pairs="adjacent", stream=None):
+    """qk_norm_rope with the keys, and the values as they are, written to the
+    cache: token t to position positions[t] of table row seqs[t] (None: row t)."""
+    code, device, dim, kh = _act(q, "q"), kv.device, kv.dim, kv.kv_heads
+    _here(device)
+    if q.dim() != 3:
+        raise _bad("q must be [tokens, heads, dim]")
+    qh = q.shape[1]
+    a, b = _rows(q, qh, dim, code, device, "q"), _rows(k, kh, dim, code, device, "k")
+    c, d = _rows(v, kh, dim, code, device, "v"), _rows(q_out, qh, dim, code, device, "q_out")
+    n = _tokens_of(a, b, c, d)
+    norm = _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device)
+    check(lib().tir_qk_norm_rope_append(a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1], kv.ref,
+                                        _ints(seqs, n, device, "seqs"), _ints(positions, n, device, "positions"), n,
+                                        qh, code, C.addressof(norm), _stream(stream)))
+
+
+def kv_append(kv, k, v, seqs, positions, stream=None):
+    """Rows k, v [tokens, kv_heads, dim] to the cache, rounded or quantised."""
+    code, device = _act(k, "k"), kv.device
+    _here(device)
+    a = _rows(k, kv.kv_heads, kv.dim, code, device, "k")
+    b = _rows(v, kv.kv_heads, kv.dim, code, device, "v")
+    n = _tokens_of(a, b)
+    check(lib().tir_kv_append(kv.ref, a[0], a[1], b[0], b[1], _ints(seqs, n, device, "seqs"),
+                              _ints(positions, n, device, "positions"), n, code, _stream(stream)))
+
+
+def kv_gather(kv, k_out, v_out, seqs, positions, stream=None):
+    """Cached positions back as rows k_out, v_out [tokens, kv_heads, dim]."""
+    code, device = _act(k_out, "k_out"), kv.device
+    _here(device)
+    a = _rows(k_out, kv.kv_heads, kv.dim, code, device, "k_out")
+    b = _rows(v_out, kv.kv_heads, kv.dim, code, device, "v_out")
+    n = _tokens_of(a, b)
+    check(lib().tir_kv_gather(kv.ref, a[0], a[1], b[0], b[1], _ints(seqs, n, device, "seqs"),
+                              _ints(positions, n, device, "positions"), n, code, _stream(stream)))
+
+
+def paged_attention_workspace(kv, rows, q_heads, max_len=0, window=0):
+    """Bytes of workspace paged_attention needs for these sizes (0: none)."""
+    n = int(lib().tir_paged_attention_workspace(kv.ref, rows, q_heads, max_len, window))
+    if n < 0:
+        raise _bad(lib().tir_last_error().decode(errors="replace"))
+    return n
+
+
+def paged_attention(q, kv, seq_lens, out, scale=0.0, max_len=0, window=0, workspace=None, stream=None):
+    """One query token per sequence over its pages: row r of q [rows, q_heads, dim]
+    over the last `window` (0: all) of the seq_lens[r] positions of table row r;
+    zeros for a row of length 0.  workspace: a uint8 tensor of
+    paged_attention_workspace bytes; without one it is taken from torch's allocator
+    for the call, on the current stream."""
+    code, device = _act(q, "q"), kv.device
+    _here(device)
+    if q.dim() != 3:
+        raise _bad("q must be [rows, q_heads, dim]")
+    qh = q.shape[1]
+    a, b = _rows(q, qh, kv.dim, code, device, "q"), _rows(out, qh, kv.dim, code, device, "out")
+    n = _tokens_of(a, b)
+    if workspace is None:
+        size = paged_attention_workspace(kv, n, qh, max_len, window)
+        if size:
+            import torch
+            if stream is not None and _stream(stream) != torch.cuda.current_stream().cuda_stream:
+                raise _bad("paged_attention on another stream than the current one needs a workspace")
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != device or not workspace.is_contiguous():
+        raise _bad(f"workspace must be a contiguous tensor on device {device}")
+    check(lib().tir_paged_attention(a[0], a[1], kv.ref, _ints(seq_lens, n, device, "seq_lens"), b[0], b[1], n, qh,
+                                    code, scale, max_len, window, _ptr(workspace),
+                                    workspace.numel() * workspace.element_size() if workspace is not None else 0,
+                                    _stream(stream)))
