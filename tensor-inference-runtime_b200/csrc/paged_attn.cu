@@ -1,93 +1,134 @@
-// paged_attn.cu -- attention of one query token per sequence over its pages.
-//
-// One warp per (row, query head): every lane holds dim / 32 neighbouring
-// elements of the query and the running output; the scores of a position are a
-// warp sum, the softmax keeps a running maximum and sum (base 2) in f32.
+// paged_attn.cu -- tir_paged_attention: the choice of kernel and split, and the
+// kernel that joins the parts of rows shared by several CTAs.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <string>
 
-#include "paged.cuh"
-#include "paged.h"
+#include "launch.cuh"
+#include "paged_attn.cuh"
 
 namespace tir {
 
 namespace {
 
-constexpr uint32_t FULL = 0xffffffffu;
+constexpr int kJoinWarps = 4;
 
-struct AttnArgs {
-    const char* q;
-    char* out;
-    int64_t q_stride, out_stride;  // elements
-    const int32_t* lens;
-    int64_t rows;
-    int32_t q_heads, group;
-    int32_t window;  // INT32_MAX: none
-    float scale_log2;
-    Elem act, cache;
-};
-
-__device__ __forceinline__ float load_elem(const char* p, int64_t i, Elem e) {
-    if (e == Elem::F32) return reinterpret_cast<const float*>(p)[i];
-    if (e == Elem::F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
-    return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-}
-
-__device__ __forceinline__ float load_cached(const char* pool, const uint16_t* steps, int64_t i, Elem e) {
-    if (e == Elem::Q8)
-        return __fmul_rn(static_cast<float>(reinterpret_cast<const int8_t*>(pool)[i]),
-                         __half2float(__ushort_as_half(steps[i >> 5])));
-    return load_elem(pool, i, e);
-}
-
+// o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the parts of one (row,
+// head).  A CTA per head; warp w takes parts w, w + 4, ..., lanes the dimensions.
+// Reads what the split wrote (L2), a few percent of the cache's bytes at most.
 template <int D>
-__global__ void __launch_bounds__(32) attn_kernel(const AttnArgs a, const PagesView kv) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join(const AttnArgs a, const PagesView kv, int32_t unit) {
     constexpr int N = D / 32;
+    __shared__ float part[kJoinWarps][D];
+    __shared__ float sums[kJoinWarps];
+    griddep_wait();
     const int64_t row = blockIdx.x / a.q_heads;
     const int h = static_cast<int>(blockIdx.x % a.q_heads);
-    const int g = h / a.group, lane = threadIdx.x;
-    const int64_t cap = static_cast<int64_t>(kv.max_pages) * kv.page_size;
-    int32_t len = a.lens[row];
-    if (len < 0 || len > cap) {
-        if (lane == 0) atomicOr(kv.err, kBadLength);
-        len = len < 0 ? 0 : static_cast<int32_t>(cap);
-    }
-    float q[N], o[N], m = -INFINITY, l = 0.f;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const AttnRange range = attn_range(row_length(a, kv, row), a.window, a.splits, a.min_units, unit, 0);
+    if (range.used <= 1) return;  // written by the split itself
+    const float* ml = a.part_ml + (row * a.q_heads + h) * a.splits * 2;
+    const float* po = a.part_o + (row * a.q_heads + h) * a.splits * D + lane * N;
+    float top = -INFINITY;
+    for (int i = lane; i < range.used; i += 32) top = fmaxf(top, ml[2 * i]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        q[i] = load_elem(a.q, row * a.q_stride + h * D + lane * N + i, a.act) * a.scale_log2;
-        o[i] = 0.f;
-    }
-    for (int32_t pos = len > a.window ? len - a.window : 0; pos < len; ++pos) {
-        const int32_t id = page_of(kv, row, pos);
-        if (id < 0) continue;
-        const int64_t at = slot_of(kv, id, pos) + g * kv.head_stride + lane * N;
-        float s = 0.f;
+    for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    float o[N], l = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) s = fmaf(q[i], load_cached(kv.k, kv.ks, at + i, a.cache), s);
+    for (int e = 0; e < N; ++e) o[e] = 0.f;
+#pragma unroll 4
+    for (int i = warp; i < range.used; i += kJoinWarps) {
+        const float2 x = *reinterpret_cast<const float2*>(ml + 2 * i);
+        const float f = x.x == -INFINITY ? 0.f : exp2_fast(x.x - top);
+        l = fmaf(f, x.y, l);
 #pragma unroll
-        for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(FULL, s, w);
-        const float mn = fmaxf(m, s), safe = mn == -INFINITY ? 0.f : mn;
-        const float corr = exp2f(m - safe), p = exp2f(s - safe);
-        l = l * corr + p;
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = fmaf(p, load_cached(kv.v, kv.vs, at + i, a.cache), o[i] * corr);
-        m = mn;
+        for (int e = 0; e < N; e += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(po + static_cast<int64_t>(i) * D + e);
+            o[e] = fmaf(f, v.x, o[e]);
+            o[e + 1] = fmaf(f, v.y, o[e + 1]);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float r = len == 0 ? 0.f : o[i] / l;
-        const int64_t at = row * a.out_stride + h * D + lane * N + i;
+    for (int e = 0; e < N; ++e) part[warp][lane * N + e] = o[e];
+    if (lane == 0) sums[warp] = l;
+    __syncthreads();
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) sum += sums[w];
+    for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
+        float y = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) y += part[w][d];
+        y /= sum;
+        const int64_t at = row * a.out_stride + static_cast<int64_t>(h) * D + d;
         if (a.act == Elem::F32)
-            reinterpret_cast<float*>(a.out)[at] = r;
+            reinterpret_cast<float*>(a.out)[at] = y;
         else if (a.act == Elem::F16)
-            reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(r);
+            reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(y);
         else
-            reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(r);
+            reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
     }
+}
+
+cudaError_t attn(const AttnArgs* a, const PagesView& kv, Elem cache, bool f32q, int nt, int64_t rows, cudaStream_t st,
+                 AttnShape* shape) {
+    switch (cache) {
+        case Elem::F32: return attn_f32(a, kv, nt, rows, st, shape);
+        case Elem::F16: return attn_f16(a, kv, f32q, nt, rows, st, shape);
+        case Elem::BF16: return attn_bf16(a, kv, f32q, nt, rows, st, shape);
+        default: return attn_q8(a, kv, f32q, nt, rows, st, shape);
+    }
+}
+
+int multiprocessors() {
+    static thread_local int dev_of = -1, n_of = 0;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev != dev_of) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        dev_of = dev;
+        n_of = n;
+    }
+    return n_of;
+}
+
+struct Plan {
+    int nt, head_tiles;
+    AttnShape shape;
+    int32_t splits, min_units;
+};
+
+// How many CTAs share a row: enough to fill the GPU twice over, and parts of at
+// most 32 units, so that rows of unequal length even out; none below two units.
+tir_status make_plan(const PagesView& kv, Elem cache, bool f32q, int64_t rows, int32_t q_heads, int64_t max_len,
+                     int64_t window, Plan* p) {
+    const int group = q_heads / kv.kv_heads;
+    p->nt = group <= 8 ? 1 : 2;
+    p->head_tiles = (group + 8 * p->nt - 1) / (8 * p->nt);
+    attn(nullptr, kv, cache, f32q, p->nt, rows, nullptr, &p->shape);
+    const int sms = multiprocessors();
+    if (sms <= 0) return fail(TIR_ERR_CUDA, "tir_paged_attention: no multiprocessor count for the current device");
+    int64_t n = static_cast<int64_t>(kv.max_pages) * kv.page_size;
+    if (max_len > 0) n = std::min(n, max_len);
+    if (window > 0) n = std::min(n, window);
+    const int64_t units = (n + p->shape.unit - 1) / p->shape.unit;
+    const int64_t base = std::max<int64_t>(rows * kv.kv_heads * p->head_tiles, 1);
+    const int64_t slots = static_cast<int64_t>(sms) * p->shape.per_sm;
+    p->min_units = 2;
+    int64_t splits = std::max((2 * slots + base - 1) / base, (units + 31) / 32);
+    splits = std::min(splits, (units + p->min_units - 1) / p->min_units);
+    splits = std::max<int64_t>(splits, 1);
+    if (base * splits > INT32_MAX) return fail(TIR_ERR_UNSUPPORTED_SHAPE, "tir_paged_attention: too many rows");
+    p->splits = static_cast<int32_t>(splits);
+    return TIR_OK;
+}
+
+int64_t workspace_of(const Plan& p, int64_t rows, int32_t q_heads, int32_t dim) {
+    return p.splits > 1 ? rows * q_heads * p.splits * (dim + 2) * 4 : 0;
 }
 
 }  // namespace
@@ -115,7 +156,14 @@ int64_t tir_paged_attention_workspace(const tir_kv_pages* kv, int64_t rows, int3
     Elem cache;
     PagesView view;
     if (check_sizes(kv, rows, q_heads, max_len, window, &view, &cache) != TIR_OK) return -1;
-    return 0;
+    // the query type may change the kernel's geometry: what either would need
+    int64_t most = 0;
+    for (const bool f32q : {false, true}) {
+        Plan p;
+        if (make_plan(view, cache, f32q, rows, q_heads, max_len, window, &p) != TIR_OK) return -1;
+        most = std::max(most, workspace_of(p, rows, q_heads, kv->dim));
+    }
+    return most;
 }
 
 tir_status tir_paged_attention(const void* q, int64_t q_stride, const tir_kv_pages* kv, const int32_t* seq_lens,
@@ -123,8 +171,6 @@ tir_status tir_paged_attention(const void* q, int64_t q_stride, const tir_kv_pag
                                float scale, int64_t max_len, int64_t window, void* workspace, int64_t workspace_bytes,
                                void* stream) {
     clear_error();
-    (void)workspace;
-    (void)workspace_bytes;
     const char* who = "tir_paged_attention";
     Elem act, cache;
     PagesView view;
@@ -141,29 +187,36 @@ tir_status tir_paged_attention(const void* q, int64_t q_stride, const tir_kv_pag
     if (rc != TIR_OK) return rc;
     rc = paged_error_word(&view.err);
     if (rc != TIR_OK) return rc;
+    Plan p;
+    rc = make_plan(view, cache, act == Elem::F32, rows, q_heads, max_len, window, &p);
+    if (rc != TIR_OK) return rc;
+    const int64_t need = workspace_of(p, rows, q_heads, kv->dim);
+    if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+        return fail(TIR_ERR_INVALID_ARG, std::string(who) + ": needs a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
     AttnArgs a{};
     a.q = static_cast<const char*>(q);
     a.out = static_cast<char*>(out);
     a.q_stride = q_stride;
     a.out_stride = out_stride;
     a.lens = seq_lens;
-    a.rows = rows;
     a.q_heads = q_heads;
     a.group = q_heads / kv->kv_heads;
+    a.head_tiles = p.head_tiles;
     a.window = window > 0 && window < INT32_MAX ? static_cast<int32_t>(window) : INT32_MAX;
+    a.splits = p.splits;
+    a.min_units = p.min_units;
     const float sc = scale == 0.f ? 1.0f / std::sqrt(static_cast<float>(kv->dim)) : scale;
     a.scale_log2 = sc * 1.44269504088896340736f;
     a.act = act;
-    a.cache = cache;
-    const unsigned grid = static_cast<unsigned>(rows * q_heads);
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + (need > 0 ? rows * q_heads * p.splits * kv->dim : 0);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (kv->dim == 64)
-        attn_kernel<64><<<grid, 32, 0, st>>>(a, view);
-    else if (kv->dim == 128)
-        attn_kernel<128><<<grid, 32, 0, st>>>(a, view);
-    else
-        attn_kernel<256><<<grid, 32, 0, st>>>(a, view);
-    const cudaError_t e = cudaGetLastError();
+    cudaError_t e = attn(&a, view, cache, act == Elem::F32, p.nt, rows, st, nullptr);
+    if (e == cudaSuccess && p.splits > 1) {
+        const dim3 grid(static_cast<unsigned>(rows * q_heads)), block(kJoinWarps * 32);
+        auto* join = kv->dim == 64 ? paged_attn_join<64> : kv->dim == 128 ? paged_attn_join<128> : paged_attn_join<256>;
+        e = launch_kernel(join, grid, block, 0, st, true, a, view, static_cast<int32_t>(p.shape.unit));
+    }
     return e == cudaSuccess ? TIR_OK : paged_fail(e, who);
 }
 

@@ -1,0 +1,741 @@
+// paged_attn.cuh -- decode attention over a paged cache: one query token per
+// sequence, a group of query heads per key-value head.
+//
+//   t_j = c (q . k_j),  c = scale log2 e;   o = sum_j 2^(t_j - m) v_j / sum_j 2^(t_j - m)
+//
+// It is bound by the bytes of the cache, read once: a key-value head's query
+// heads share every key and value.  A CTA takes one (row, key-value head, tile of
+// 8 NT query heads) over a part of the row's positions; its warps take tiles of
+// 16 positions in turn, each with a ring of cp.async stages and a softmax
+// (m, l, o) of its own, so the loop has no CTA barrier.  The parts meet in shared
+// memory, those of different CTAs in paged_attn_join.
+//
+// Products on the tensor cores (mma.sync: with 8 query heads a tile is M = 16
+// positions or dimensions by N = 8 heads, far below the smallest tcgen05 tile,
+// and the pipe is not the bound), transposed so that heads are the N columns and
+// no row of a tile is padding:
+//   S' (16 positions x 8 heads)  = K (16 x dim) . Q' (dim x 8)
+//   O' (dim x 8 heads)          += V' (dim x 16) . P' (16 x 8)
+// S' comes out with positions along the lanes' rows; movmatrix turns its 8 x 8
+// blocks into the operand layout of P'.
+//
+// Operand types.  K and V enter as they are stored: f16 / bf16 directly, Q8_0
+// quants as f16 integers (exact) with the block steps applied outside, f32 split
+// into two tf32 parts.  q and the weights p are split into as many parts as they
+// need: 16-bit queries are exact in one (bf16 ones scaled by a power of two for
+// f16), f32 queries take two f16 (22 bits under a per-head power of two), three
+// bf16 or two tf32 parts; p always keeps 16 bits or more (two parts; three bf16
+// under f32 queries), below the rounding of the output.  Scores, m, l and o are
+// f32 throughout.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include "paged.cuh"
+#include "ptx.cuh"
+
+namespace tir {
+
+struct AttnArgs {
+    const char* q;
+    char* out;
+    int64_t q_stride, out_stride;  // elements
+    const int32_t* lens;
+    int32_t q_heads, group, head_tiles;  // head_tiles: tiles of 8 NT query heads per key-value head
+    int32_t window;                      // INT32_MAX: none
+    int32_t splits, min_units;
+    float scale_log2;
+    Elem act;
+    float *part_o, *part_ml;  // [rows][q_heads][splits][dim], [..][splits][2]
+};
+
+constexpr int kAttnTile = 16;  // positions of a warp's tile
+
+// The part of a row's positions that split `i` of `splits` takes, in units of
+// `unit` positions: as even as whole units allow, none below `min_units` units.
+// `used` splits have any.
+struct AttnRange {
+    int32_t first, k0, k1, used;
+};
+
+__device__ __forceinline__ AttnRange attn_range(int32_t len, int32_t window, int32_t splits, int32_t min_units,
+                                                int32_t unit, int32_t i) {
+    AttnRange r;
+    r.first = len > window ? len - window : 0;
+    const int32_t units = (len - r.first + unit - 1) / unit;
+    const int32_t per = max((units + splits - 1) / splits, min_units);
+    r.used = (units + per - 1) / per;
+    const int64_t k0 = r.first + static_cast<int64_t>(i) * per * unit;
+    r.k0 = static_cast<int32_t>(min(k0, static_cast<int64_t>(len)));
+    r.k1 = static_cast<int32_t>(min(k0 + static_cast<int64_t>(per) * unit, static_cast<int64_t>(len)));
+    return r;
+}
+
+__device__ __forceinline__ int32_t row_length(const AttnArgs& a, const PagesView& kv, int64_t row) {
+    const int32_t len = a.lens[row];
+    const int64_t cap = static_cast<int64_t>(kv.max_pages) * kv.page_size;
+    if (len >= 0 && len <= cap) return len;
+    if (threadIdx.x == 0) atomicOr(kv.err, kBadLength);
+    return len < 0 ? 0 : static_cast<int32_t>(cap);
+}
+
+// ---- instruction wrappers ----------------------------------------------------
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+template <int B>
+__device__ __forceinline__ void cp_async_small_or_zero(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(B), "r"(live ? B : 0)
+                 : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void ldsm4_t(uint32_t* r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// d (16 x 8, f32) += a (16 x 16) b (16 x 8)
+template <bool BF>
+__device__ __forceinline__ void mma16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if constexpr (BF)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// d (16 x 8, f32) += a (16 x 8) b (8 x 8), tf32 operands
+__device__ __forceinline__ void mma8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t to_tf32(float x) {
+    uint32_t y;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
+    return y;
+}
+
+// x = hi + lo to 22 bits, both tf32.
+__device__ __forceinline__ void split_tf32(float x, uint32_t* hi, uint32_t* lo) {
+    *hi = to_tf32(x);
+    *lo = to_tf32(x - __uint_as_float(*hi));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two int8 of `w` picked by `sel` (biased bytes) as exact f16 integers: the byte
+// 128 + n under the exponent of 1024 reads 1152 + n.
+__device__ __forceinline__ uint32_t q8_pair(uint32_t w_biased, uint32_t sel) {
+    const uint32_t x = __byte_perm(w_biased, 0x64646464u, sel);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ---- configuration -----------------------------------------------------------
+// C: cache type; D: head size; NT: tiles of 8 query heads a CTA takes; F32Q: f32
+// queries (else 16-bit ones).
+template <Elem C, int D, int NT, bool F32Q>
+struct AttnCfg {
+    static constexpr bool tf32 = C == Elem::F32, bf = C == Elem::BF16, q8 = C == Elem::Q8;
+    static constexpr int ES = ElemOf<C>::bytes;
+    static constexpr int NQ = tf32 ? 2 : !F32Q ? 1 : bf ? 3 : 2;  // parts of q
+    static constexpr int NP = tf32 ? 2 : bf && F32Q ? 3 : 2;      // parts of p
+    // f16 operands hold q under a per-head power of two, but for f16 queries of f16 caches (exact as they are)
+    static constexpr bool scaled = q8 || (C == Elem::F16 && F32Q);
+    static constexpr int ROW = D * ES;
+    static constexpr int PITCH = ROW + 16;  // an odd number of 16-byte units: ldmatrix rows fall on different banks
+    static constexpr int STEPS = q8 ? D / 32 * 2 : 0;  // bytes of a position's Q8_0 steps
+    static constexpr int V_AT = kAttnTile * PITCH;
+    static constexpr int KS_AT = 2 * kAttnTile * PITCH, VS_AT = KS_AT + kAttnTile * STEPS;
+    static constexpr int STAGE = KS_AT + 2 * kAttnTile * STEPS;
+    static constexpr int KSTEPS = tf32 ? D / 8 : D / 16;  // q operand steps
+    static constexpr int QBYTES = KSTEPS * NT * NQ * 256;
+    static constexpr int HEADS = 8 * NT;
+    static constexpr int WARPS = STAGE > 32 * 1024 ? 2 : 4;
+    static constexpr int THREADS = WARPS * 32;
+    static constexpr int UNIT = WARPS * kAttnTile;
+    static constexpr int FIXED = QBYTES + HEADS * 4 + WARPS * HEADS * 8;
+    // two CTAs an SM where three stages fit in half of its shared memory, else one
+    static constexpr int half_stages = (112 * 1024 - FIXED) / (WARPS * STAGE);
+    static constexpr int full_stages = (224 * 1024 - FIXED) / (WARPS * STAGE);
+    static constexpr int PER_SM = half_stages >= 3 ? 2 : 1;
+    static constexpr int fit = PER_SM == 2 ? half_stages : full_stages;
+    static constexpr int STAGES = fit > 6 ? 6 : fit;
+    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int SMEM = RING + FIXED;
+    // q operands in registers where they are few
+    static constexpr bool q_in_regs = KSTEPS * NT * NQ * 2 <= 64;
+    static_assert(STAGES >= 2 && SMEM <= 227 * 1024, "the ring needs two stages");
+    static_assert(STAGES * STAGE >= HEADS * (D + 4) * 4, "a warp's output fits its ring");
+    static_assert(STAGE % 16 == 0 && RING % 16 == 0 && QBYTES % 16 == 0, "16-byte copies");
+};
+
+template <Elem C, int D, int NT, bool F32Q>
+__global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D, NT, F32Q>::PER_SM)
+    paged_attn_kernel(const AttnArgs a, const PagesView kv) {
+    using X = AttnCfg<C, D, NT, F32Q>;
+    constexpr uint32_t FULL = 0xffffffffu;
+    constexpr int CH = X::ROW / 16;  // 16-byte pieces of a cached row
+    // weights are kept 2^6 above their logarithm's reference, and the reference may
+    // lag the maximum by 8: f16 parts then lose nothing to the end of its range
+    constexpr float kLift = X::tf32 || X::bf ? 0.f : 6.f;
+    constexpr float kLag = 8.f;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint8_t* ring = smem;
+    uint32_t* qf = reinterpret_cast<uint32_t*>(smem + X::RING);
+    float* cs = reinterpret_cast<float*>(smem + X::RING + X::QBYTES);
+    float* ml = cs + X::HEADS;  // [WARPS][HEADS][2]
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int tiles = kv.kv_heads * a.head_tiles;
+    const int split = static_cast<int>(blockIdx.x % a.splits);
+    const unsigned rest = blockIdx.x / a.splits;
+    const int64_t row = rest / tiles;
+    const int hk = static_cast<int>(rest % tiles) / a.head_tiles;
+    const int j0 = static_cast<int>(rest % tiles) % a.head_tiles * X::HEADS;  // first head of the group
+    const int nh = min(a.group - j0, X::HEADS);
+    const int h0 = hk * a.group + j0;
+    const int32_t len = row_length(a, kv, row);
+    const AttnRange range = attn_range(len, a.window, a.splits, a.min_units, X::UNIT, split);
+    if (range.used == 0) {  // nothing to look at: zeros
+        if (split == 0)
+            for (int i = threadIdx.x; i < nh * (D / 8); i += X::THREADS) {
+                const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                const int64_t at = row * a.out_stride + static_cast<int64_t>(h0) * D + i * 8;
+                if (a.act == Elem::F32)
+                    store8_as<Elem::F32>(a.out + at * 4, z);
+                else
+                    store8_as<Elem::F16>(a.out + at * 2, z);
+            }
+        return;
+    }
+    if (range.k0 >= range.k1) return;
+
+    // ---- the ring ----
+    const int n_tiles = (range.k1 - range.k0 + kAttnTile - 1) / kAttnTile;
+    const int my_tiles = n_tiles > warp ? (n_tiles - warp + X::WARPS - 1) / X::WARPS : 0;
+    uint8_t* my_ring = ring + warp * X::STAGES * X::STAGE;
+    const uint32_t ring_addr = smem_u32(my_ring);
+    // page of this lane's position (lane % 16) of the warp's tile i; -1 past the end
+    auto lookup = [&](int i) -> int32_t {
+        const int32_t pos = range.k0 + (i * X::WARPS + warp) * kAttnTile + (lane & 15);
+        return i < my_tiles && pos < range.k1 ? page_of(kv, row, pos) : -1;
+    };
+    const int64_t head_at = static_cast<int64_t>(hk) * kv.head_stride;
+    auto issue = [&](int i, int32_t page) {
+        if (i < my_tiles) {
+            const int32_t pos = range.k0 + (i * X::WARPS + warp) * kAttnTile + (lane & 15);
+            const int64_t mine = page < 0 ? -1 : slot_of(kv, page, pos) + head_at;
+            const uint32_t dst = ring_addr + (i % X::STAGES) * X::STAGE;
+            if constexpr (X::q8) {
+                const bool live = mine >= 0;
+                const uint16_t* src = (lane < 16 ? kv.ks : kv.vs) + (live ? mine >> 5 : 0);
+                cp_async_small_or_zero<X::STEPS>(dst + (lane < 16 ? X::KS_AT : X::VS_AT) + (lane & 15) * X::STEPS, src, live);
+            }
+#pragma unroll
+            for (int u = 0; u < kAttnTile * CH / 32; ++u) {
+                const int idx = u * 32 + lane, key = idx / CH, ch = idx % CH;
+                const int64_t at = __shfl_sync(FULL, mine, key);
+                const bool live = at >= 0;
+                const int64_t byte = (live ? at : 0) * X::ES + ch * 16;
+                const uint32_t to = dst + key * X::PITCH + ch * 16;
+                cp_async16_or_zero(to, kv.k + (live ? byte : 0), live);
+                cp_async16_or_zero(to + X::V_AT, kv.v + (live ? byte : 0), live);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < X::STAGES - 1; ++i) issue(i, lookup(i));
+    int32_t next_page = lookup(X::STAGES - 1);
+
+    // ---- q operands, while the first tiles are on their way ----
+    for (int j = warp; j < X::HEADS; j += X::WARPS) {
+        float x[D / 32];
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            x[i] = 0.f;
+            if (j < nh) {
+                const int64_t at = row * a.q_stride + static_cast<int64_t>(h0 + j) * D + i * 32 + lane;
+                x[i] = a.act == Elem::F32   ? reinterpret_cast<const float*>(a.q)[at]
+                       : a.act == Elem::F16 ? __half2float(reinterpret_cast<const __half*>(a.q)[at])
+                                            : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.q)[at]);
+            }
+            top = fmaxf(top, fabsf(x[i]));
+        }
+        float c = a.scale_log2;
+        if constexpr (X::scaled) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
+            const int e = static_cast<int>(__float_as_uint(top) >> 23);  // biased exponent
+            if (e > 0 && e < 255) {                                      // top * 2^s in [2^9, 2^10)
+                const int s = min(136 - e, 120);
+                const float up = __uint_as_float(static_cast<uint32_t>(127 + s) << 23);
+                c *= __uint_as_float(static_cast<uint32_t>(127 - s) << 23);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) x[i] *= up;
+            }
+        }
+        if (lane == 0) cs[j] = c;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int e = i * 32 + lane;  // element of the head
+            if constexpr (X::tf32) {
+                const int kk = e / 8, r = e % 8, at = ((kk * NT + j / 8) * 2) * 64 + ((j % 8) * 4 + r % 4) * 2 + r / 4;
+                split_tf32(x[i], &qf[at], &qf[at + 64]);
+            } else {
+                // operand element k = 2 t' + {0, 1} (+ 8 in the second register); Q8_0 words
+                // hold elements 4 t' .. 4 t' + 3, so there the order inside 16 is theirs
+                const int kk = e / 16, r = e % 16;
+                const int tt = X::q8 ? r / 4 : r % 8 / 2, reg = X::q8 ? r % 4 / 2 : r / 8;
+                float rem = x[i];
+#pragma unroll
+                for (int s = 0; s < X::NQ; ++s) {
+                    const int at = (((kk * NT + j / 8) * X::NQ + s) * 32 + (j % 8) * 4 + tt) * 2 + reg;
+                    uint16_t* p = reinterpret_cast<uint16_t*>(qf + at) + (r & 1);
+                    if constexpr (X::bf) {
+                        const __nv_bfloat16 b = __float2bfloat16_rn(rem);
+                        *p = __bfloat16_as_ushort(b);
+                        rem -= __bfloat162float(b);
+                    } else {
+                        const __half b = __float2half_rn(rem);
+                        *p = __half_as_ushort(b);
+                        rem -= __half2float(b);
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    uint32_t qr[X::q_in_regs ? X::KSTEPS * NT * X::NQ * 2 : 1];
+    if constexpr (X::q_in_regs) {
+#pragma unroll
+        for (int i = 0; i < X::KSTEPS * NT * X::NQ; ++i) {
+            const uint2 w = reinterpret_cast<const uint2*>(qf)[i * 32 + lane];
+            qr[2 * i] = w.x;
+            qr[2 * i + 1] = w.y;
+        }
+    }
+    auto q_op = [&](int kk, int nt, int s) -> uint2 {
+        const int i = (kk * NT + nt) * X::NQ + s;
+        if constexpr (X::q_in_regs) return make_uint2(qr[2 * i], qr[2 * i + 1]);
+        else return reinterpret_cast<const uint2*>(qf)[i * 32 + lane];
+    };
+    float c[NT][2], m[NT][2], l[NT][2], o[D / 16][NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            c[n][e] = cs[n * 8 + 2 * t + e];
+            m[n][e] = -INFINITY;
+            l[n][e] = 0.f;
+        }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+    int v_exp = 0;  // Q8_0: o is kept over 2^(v_exp - 14), the power of two above the steps seen so far
+
+    // ---- the loop over this warp's tiles ----
+    for (int it = 0; it < my_tiles; ++it) {
+        cp_async_wait<X::STAGES - 2>();
+        __syncwarp();
+        issue(it + X::STAGES - 1, next_page);
+        next_page = lookup(it + X::STAGES);
+        const uint8_t* st = my_ring + (it % X::STAGES) * X::STAGE;
+        const uint32_t sa = ring_addr + (it % X::STAGES) * X::STAGE;
+        const uint32_t row_addr = sa + (lane & 15) * X::PITCH + (lane >> 4) * 16;
+
+        // S' = K Q'
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+        if constexpr (X::q8) {
+            uint16_t k_steps[2][D / 32];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int b = 0; b < D / 32; ++b)
+                    k_steps[half][b] = reinterpret_cast<const uint16_t*>(st + X::KS_AT)[(g + 8 * half) * (D / 32) + b];
+#pragma unroll
+            for (int b = 0; b < D / 32; ++b) {
+                uint32_t w[4], x0[4], x1[4];
+                ldsm4(w, row_addr + b * 32);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
+                x0[0] = q8_pair(w[0], 0x4140), x0[1] = q8_pair(w[1], 0x4140);
+                x0[2] = q8_pair(w[0], 0x4342), x0[3] = q8_pair(w[1], 0x4342);
+                x1[0] = q8_pair(w[2], 0x4140), x1[1] = q8_pair(w[3], 0x4140);
+                x1[2] = q8_pair(w[2], 0x4342), x1[3] = q8_pair(w[3], 0x4342);
+                const float d0 = __half2float(__ushort_as_half(k_steps[0][b])), d1 = __half2float(__ushort_as_half(k_steps[1][b]));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int p = X::NQ - 1; p >= 0; --p) {
+                        const uint2 q0 = q_op(2 * b, n, p), q1 = q_op(2 * b + 1, n, p);
+                        mma16<false>(acc, x0, q0.x, q0.y);
+                        mma16<false>(acc, x1, q1.x, q1.y);
+                    }
+                    s[n][0] = fmaf(acc[0], d0, s[n][0]);
+                    s[n][1] = fmaf(acc[1], d0, s[n][1]);
+                    s[n][2] = fmaf(acc[2], d1, s[n][2]);
+                    s[n][3] = fmaf(acc[3], d1, s[n][3]);
+                }
+            }
+        } else if constexpr (X::tf32) {
+            float s2[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s2[n][e] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < D / 8; ++kk) {
+                uint32_t w[4], hi[4], lo[4];
+                ldsm4(w, row_addr + kk * 32);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split_tf32(__uint_as_float(w[e]), &hi[e], &lo[e]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint2 qh = q_op(kk, n, 0), ql = q_op(kk, n, 1);
+                    mma8(s2[n], lo, qh.x, qh.y);
+                    mma8(s2[n], hi, ql.x, ql.y);
+                    mma8(s[n], hi, qh.x, qh.y);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
+        } else {
+            float s2[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s2[n][e] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                uint32_t w[4];
+                ldsm4(w, row_addr + kk * 32);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int p = X::NQ - 1; p >= 0; --p) {
+                        const uint2 qv = q_op(kk, n, p);
+                        mma16<X::bf>(((kk + p) & 1) ? s2[n] : s[n], w, qv.x, qv.y);
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
+        }
+
+        // weights: p = 2^(t - m + lift), with m moved only when a score passes it by
+        // more than kLag (rare after the first tiles): no reduction in the usual tile
+        const int32_t key0 = range.k0 + (it * X::WARPS + warp) * kAttnTile + g;
+        bool moves = false;
+        float top[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                s[n][e] = key0 < range.k1 ? s[n][e] * c[n][e] : -INFINITY;
+                s[n][e + 2] = key0 + 8 < range.k1 ? s[n][e + 2] * c[n][e] : -INFINITY;
+                top[n][e] = fmaxf(s[n][e], s[n][e + 2]);
+                moves |= top[n][e] > m[n][e] + kLag;
+            }
+        uint32_t v_top = 0u;
+        uint16_t v_steps[2][X::q8 ? D / 32 : 1];
+        if constexpr (X::q8) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int b = 0; b < D / 32; ++b) {
+                    v_steps[half][b] = reinterpret_cast<const uint16_t*>(st + X::VS_AT)[(g + 8 * half) * (D / 32) + b];
+                    v_top = max(v_top, static_cast<uint32_t>(v_steps[half][b] & 0x7fffu) >> 10);
+                }
+            moves |= static_cast<int>(v_top) > v_exp;
+        }
+        if (__any_sync(FULL, moves)) {
+            float shrink = 1.f;
+            if constexpr (X::q8) {
+#pragma unroll
+                for (int w = 16; w; w >>= 1) v_top = max(v_top, __shfl_xor_sync(FULL, v_top, w));
+                const int up = max(static_cast<int>(v_top) - v_exp, 0);
+                shrink = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+                v_exp += up;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(FULL, top[n][e], w));
+                    const float mn = fmaxf(m[n][e], top[n][e]);
+                    const float corr = m[n][e] == mn ? 1.f : exp2_fast(m[n][e] - mn);
+                    m[n][e] = mn;
+                    l[n][e] *= corr;
+                    f[e] = corr * shrink;
+                }
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    o[i][n][0] *= f[0];
+                    o[i][n][1] *= f[1];
+                    o[i][n][2] *= f[0];
+                    o[i][n][3] *= f[1];
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float base = (m[n][e] == -INFINITY ? 0.f : m[n][e]) - kLift;
+                s[n][e] = exp2_fast(s[n][e] - base);
+                s[n][e + 2] = exp2_fast(s[n][e + 2] - base);
+                l[n][e] += s[n][e] + s[n][e + 2];
+            }
+
+        // O' += V' P'
+        if constexpr (X::q8) {
+            const float inv = __uint_as_float(static_cast<uint32_t>(127 + 14 - v_exp) << 23);
+#pragma unroll
+            for (int b = 0; b < D / 32; ++b) {
+                const float d0 = __half2float(__ushort_as_half(v_steps[0][b])) * inv;
+                const float d1 = __half2float(__ushort_as_half(v_steps[1][b])) * inv;
+                uint32_t p0[NT][2], p1[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float w0 = s[n][0] * d0, w1 = s[n][1] * d0, w2 = s[n][2] * d1, w3 = s[n][3] * d1;
+                    const __half2 ha = __floats2half2_rn(w0, w1), hb = __floats2half2_rn(w2, w3);
+                    const float2 fa = __half22float2(ha), fb = __half22float2(hb);
+                    p0[n][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&ha));
+                    p0[n][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hb));
+                    p1[n][0] = transpose8x8(pack2(w0 - fa.x, w1 - fa.y, Elem::F16));
+                    p1[n][1] = transpose8x8(pack2(w2 - fb.x, w3 - fb.y, Elem::F16));
+                }
+                uint32_t w[4];
+                ldsm4_t(w, sa + X::V_AT + (lane & 15) * X::PITCH + b * 32 + (lane >> 4) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t x[4];
+                    x[0] = q8_pair(w[2 * i], 0x4240), x[1] = q8_pair(w[2 * i], 0x4341);
+                    x[2] = q8_pair(w[2 * i + 1], 0x4240), x[3] = q8_pair(w[2 * i + 1], 0x4341);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16<false>(o[2 * b + i][n], x, p1[n][0], p1[n][1]);
+                        mma16<false>(o[2 * b + i][n], x, p0[n][0], p0[n][1]);
+                    }
+                }
+            }
+        } else if constexpr (X::tf32) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint32_t x = __float_as_uint(s[n][2 * kb]), y = __float_as_uint(s[n][2 * kb + 1]);
+                    const uint32_t up = transpose8x8(__byte_perm(x, y, 0x7632)), dn = transpose8x8(__byte_perm(x, y, 0x5410));
+                    split_tf32(__uint_as_float(__byte_perm(dn, up, 0x5410)), &ph[n][0], &pl[n][0]);
+                    split_tf32(__uint_as_float(__byte_perm(dn, up, 0x7632)), &ph[n][1], &pl[n][1]);
+                }
+                const uint8_t* v = st + X::V_AT + (8 * kb + 2 * t) * X::PITCH + g * 8;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const float2 va = *reinterpret_cast<const float2*>(v + i * 64);
+                    const float2 vb = *reinterpret_cast<const float2*>(v + X::PITCH + i * 64);
+                    uint32_t hi[4], lo[4];
+                    split_tf32(va.x, &hi[0], &lo[0]);
+                    split_tf32(va.y, &hi[1], &lo[1]);
+                    split_tf32(vb.x, &hi[2], &lo[2]);
+                    split_tf32(vb.y, &hi[3], &lo[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma8(o[i][n], lo, ph[n][0], ph[n][1]);
+                        mma8(o[i][n], hi, pl[n][0], pl[n][1]);
+                        mma8(o[i][n], hi, ph[n][0], ph[n][1]);
+                    }
+                }
+            }
+        } else {
+            uint32_t pp[NT][X::NP][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float r0 = s[n][0], r1 = s[n][1], r2 = s[n][2], r3 = s[n][3];
+#pragma unroll
+                for (int p = 0; p < X::NP; ++p) {
+                    const uint32_t wa = pack2(r0, r1, C), wb = pack2(r2, r3, C);
+                    pp[n][p][0] = transpose8x8(wa);
+                    pp[n][p][1] = transpose8x8(wb);
+                    const float2 fa = unpack2(wa, C), fb = unpack2(wb, C);
+                    r0 -= fa.x, r1 -= fa.y, r2 -= fb.x, r3 -= fb.y;
+                }
+            }
+            const uint32_t v_addr = sa + X::V_AT + ((lane & 7) + (lane >> 4) * 8) * X::PITCH + ((lane >> 3) & 1) * 16;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                uint32_t w[4];
+                ldsm4_t(w, v_addr + i * 32);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int p = X::NP - 1; p >= 0; --p) mma16<X::bf>(o[i][n], w, pp[n][p][0], pp[n][p][1]);
+            }
+        }
+    }
+    cp_async_wait_all();
+    griddep_launch_dependents();
+    __syncwarp();
+
+    // ---- the warps' parts joined ----
+    if constexpr (X::q8) {
+        const float f = __uint_as_float(static_cast<uint32_t>(127 + v_exp - 14) << 23);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][n][e] *= f;
+    }
+    float* mine = reinterpret_cast<float*>(my_ring);  // [HEADS][D + 4]
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int j = n * 8 + 2 * t + e;
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(FULL, l[n][e], w);
+            if (g == 0) {
+                ml[(warp * X::HEADS + j) * 2] = m[n][e];
+                ml[(warp * X::HEADS + j) * 2 + 1] = l[n][e];
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                float* at = mine + j * (D + 4) + i * 16;
+                if constexpr (X::q8 || X::tf32) {  // rows g, g + 8 of a 16-dimension tile are dimensions 2 g, 2 g + 1
+                    *reinterpret_cast<float2*>(at + 2 * g) = make_float2(o[i][n][e], o[i][n][e + 2]);
+                } else {
+                    at[g] = o[i][n][e];
+                    at[g + 8] = o[i][n][e + 2];
+                }
+            }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nh * (D / 8); i += X::THREADS) {
+        const int j = i / (D / 8), d = i % (D / 8) * 8;
+        float top = -INFINITY, sum = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < X::WARPS; ++w) top = fmaxf(top, ml[(w * X::HEADS + j) * 2]);
+#pragma unroll
+        for (int w = 0; w < X::WARPS; ++w) {
+            const float mw = ml[(w * X::HEADS + j) * 2];
+            const float f = mw == -INFINITY ? 0.f : exp2_fast(mw - top);
+            const float lw = ml[(w * X::HEADS + j) * 2 + 1];
+            sum += f * lw;
+            const float* part = reinterpret_cast<const float*>(ring + w * X::STAGES * X::STAGE) + j * (D + 4) + d;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = fmaf(f, part[e], y[e]);
+        }
+        if (range.used == 1) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = y[e] / sum;
+            const int64_t at = row * a.out_stride + static_cast<int64_t>(h0 + j) * D + d;
+            if (a.act == Elem::F32)
+                store8_as<Elem::F32>(a.out + at * 4, y);
+            else if (a.act == Elem::F16)
+                store8_as<Elem::F16>(a.out + at * 2, y);
+            else
+                store8_as<Elem::BF16>(a.out + at * 2, y);
+        } else {
+            const int64_t at = (row * a.q_heads + h0 + j) * a.splits + split;
+            store8_as<Elem::F32>(reinterpret_cast<char*>(a.part_o + at * D + d), y);
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, sum);
+        }
+    }
+}
+
+template <Elem C, int D, int NT, bool F32Q>
+cudaError_t launch_attn_as(const AttnArgs& a, const PagesView& kv, int64_t rows, cudaStream_t stream) {
+    using X = AttnCfg<C, D, NT, F32Q>;
+    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<C, D, NT, F32Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM);
+    if (e != cudaSuccess) return e;
+    const unsigned grid = static_cast<unsigned>(rows * kv.kv_heads * a.head_tiles * a.splits);
+    paged_attn_kernel<C, D, NT, F32Q><<<grid, X::THREADS, X::SMEM, stream>>>(a, kv);
+    return cudaGetLastError();
+}
+
+// Geometry of the kernel that a cache type, head size and query type get: CTAs
+// an SM holds, and the positions of a unit.
+struct AttnShape {
+    int per_sm, unit;
+};
+
+template <Elem C, int D, bool F32Q>
+AttnShape attn_shape_as(int nt) {
+    if (nt == 1) return {AttnCfg<C, D, 1, F32Q>::PER_SM, AttnCfg<C, D, 1, F32Q>::UNIT};
+    return {AttnCfg<C, D, 2, F32Q>::PER_SM, AttnCfg<C, D, 2, F32Q>::UNIT};
+}
+
+// One function per cache type (paged_attn_<type>.cu): the launch, or with `shape`
+// given only the geometry.
+template <Elem C, bool F32Q>
+cudaError_t attn_of_type(const AttnArgs* a, const PagesView& kv, int nt, int64_t rows, cudaStream_t st, AttnShape* shape) {
+    auto go = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        if (shape) {
+            *shape = attn_shape_as<C, D, F32Q>(nt);
+            return cudaSuccess;
+        }
+        return nt == 1 ? launch_attn_as<C, D, 1, F32Q>(*a, kv, rows, st) : launch_attn_as<C, D, 2, F32Q>(*a, kv, rows, st);
+    };
+    if (kv.dim == 64) return go(std::integral_constant<int, 64>{});
+    if (kv.dim == 128) return go(std::integral_constant<int, 128>{});
+    return go(std::integral_constant<int, 256>{});
+}
+
+cudaError_t attn_f32(const AttnArgs* a, const PagesView& kv, int nt, int64_t rows, cudaStream_t st, AttnShape* shape);
+cudaError_t attn_f16(const AttnArgs* a, const PagesView& kv, bool f32q, int nt, int64_t rows, cudaStream_t st, AttnShape* shape);
+cudaError_t attn_bf16(const AttnArgs* a, const PagesView& kv, bool f32q, int nt, int64_t rows, cudaStream_t st, AttnShape* shape);
+cudaError_t attn_q8(const AttnArgs* a, const PagesView& kv, bool f32q, int nt, int64_t rows, cudaStream_t st, AttnShape* shape);
+
+}  // namespace tir
