@@ -822,40 +822,53 @@ def _bad(message):
     return TirError(23, message)  # INVALID_ARG
 
 
-def _codes():
-    """torch dtype -> TIR_DTYPE_* of activations; filled on first use (torch is
-    imported only by callers that hold tensors)."""
-    if not _CODES:
+class _Torch:
+    """What the bindings below need of torch on every call, looked up once (torch
+    is imported only by callers that hold tensors)."""
+
+    def __init__(self):
         import torch
-        _CODES.update({torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16})
-    return _CODES
+        self.codes = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+        self.float32, self.int32 = torch.float32, torch.int32
+        # the current device and its current stream without the objects around them:
+        # a call's host time is of the order of its kernel's
+        self.device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        self.stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-_CODES = {}
+_torch_state = None
 
 
-def _rows(x, heads, dim, code, device, what):
+def _torch():
+    global _torch_state
+    if _torch_state is None:
+        _torch_state = _Torch()
+    return _torch_state
+
+
+def _rows(x, heads, dim, dtype, device, what):
     """Checks a [tokens, heads, dim] tensor whose heads are adjacent; returns
     (pointer, stride between tokens in elements, tokens)."""
     shape = x.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
         raise _bad(f"{what} must be [tokens, {heads}, {dim}], got {list(shape)}")
-    stride = x.stride()
-    if stride[2] != 1 or (stride[1] != dim and heads > 1):
+    s0, s1, s2 = x.stride()
+    if s2 != 1 or (s1 != dim and heads > 1):
         raise _bad(f"{what}: a token's heads must be adjacent")
-    if _codes().get(x.dtype) != code:
+    if x.dtype is not dtype:
         raise _bad(f"{what} has another type than q or k: {x.dtype}")
     if x.get_device() != device:
         raise _bad(f"{what} is not on device {device}")
-    return x.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], heads * dim), shape[0]
+    n = shape[0]
+    return x.data_ptr(), (s0 if n > 1 else max(s0, heads * dim)), n
 
 
 def _ints(x, n, device, what):
     """Pointer of a contiguous int32 tensor of at least n values (None: NULL)."""
     if x is None:
         return None
-    if x.numel() < n or x.dim() != 1 or (n > 1 and x.stride(0) != 1) or x.element_size() != 4 or \
-            x.is_floating_point():
+    if x.dim() != 1 or x.dtype is not _torch().int32 or x.shape[0] < n or (n > 1 and x.stride(0) != 1):
         raise _bad(f"{what} must be a contiguous int32 vector of {n} values")
     if x.get_device() != device:
         raise _bad(f"{what} is not on device {device}")
@@ -863,20 +876,21 @@ def _ints(x, n, device, what):
 
 
 def _act(x, what):
-    code = _codes().get(x.dtype)
+    code = _torch().codes.get(x.dtype)
     if code is None:
         raise TirError(6, f"{what}: activations must be float32, float16 or bfloat16, got {x.dtype}")
     return code
 
 
-def _here(device):
-    """The operators launch on the current device; their tensors must be there."""
+def _launch_stream(device, stream):
+    """The stream to launch on.  The operators run on the current device, and their
+    tensors must be there."""
     if device < 0:
         raise _bad("the cache and the activations must be on a CUDA device")
-    import torch
-    if device != torch.cuda.current_device():
-        raise _bad(f"the cache or activations are on device {device}, the current device is "
-                   f"{torch.cuda.current_device()}")
+    t = _torch()
+    if device != t.device():
+        raise _bad(f"the cache or activations are on device {device}, the current device is {t.device()}")
+    return t.stream(device) if stream is None else _stream(stream)
 
 
 class KVPages:
@@ -934,28 +948,37 @@ def rope_table(base, dim, n_pos):
 
 
 def _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device):
-    import torch
-    if pairs not in PAIRS:
+    code = PAIRS.get(pairs)
+    if code is None:
         raise _bad(f"pairs must be one of {sorted(PAIRS)}")
-    n_pos = rope_dim = 0
+    t = _torch()
+    n = QKNorm()
+    n.eps = eps
     if rope is not None:
-        if rope.dim() != 3 or rope.shape[2] != 2 or not rope.is_contiguous() or rope.dtype != torch.float32:
+        shape = rope.shape
+        if len(shape) != 3 or shape[2] != 2 or rope.dtype is not t.float32 or not rope.is_contiguous():
             raise _bad("rope must be a contiguous float32 [positions, rope_dim / 2, 2] table")
-        n_pos, rope_dim = rope.shape[0], 2 * rope.shape[1]
-    for w in (q_weight, k_weight):
-        if w is not None and (w.dim() != 1 or w.shape[0] != dim or w.dtype != torch.float32 or w.stride(0) != 1):
-            raise _bad(f"a norm weight must be a contiguous float32 vector of {dim}")
-    for x in (rope, q_weight, k_weight):
-        if x is not None and x.get_device() != device:
-            raise _bad(f"rotation table and weights must be on device {device}")
-    return QKNorm(_ptr(q_weight), _ptr(k_weight), _ptr(rope), n_pos, rope_dim, PAIRS[pairs], eps)
-
-
-def _tokens_of(*rows):
-    n = rows[0][2]
-    if any(r[2] != n for r in rows):
-        raise _bad("rows of different token counts")
+        if rope.get_device() != device:
+            raise _bad(f"rope is not on device {device}")
+        n.rope, n.rope_positions, n.rope_dim, n.pairs = rope.data_ptr(), shape[0], 2 * shape[1], code
+    if q_weight is not None:
+        n.q_weight = _weight(q_weight, dim, device, t)
+    if k_weight is not None:
+        n.k_weight = _weight(k_weight, dim, device, t)
     return n
+
+
+def _weight(w, dim, device, t):
+    if w.dim() != 1 or w.shape[0] != dim or w.dtype is not t.float32 or w.stride(0) != 1:
+        raise _bad(f"a norm weight must be a contiguous float32 vector of {dim}")
+    if w.get_device() != device:
+        raise _bad(f"a norm weight is not on device {device}")
+    return w.data_ptr()
+
+
+def _same(*counts):
+    if len(set(counts)) != 1:
+        raise _bad("rows of different token counts")
 
 
 def qk_norm_rope(q, k, q_out, k_out, positions, rope=None, q_weight=None, k_weight=None, eps=1e-5, pairs="adjacent",
@@ -963,58 +986,61 @@ def qk_norm_rope(q, k, q_out, k_out, positions, rope=None, q_weight=None, k_weig
     """Per-head rmsnorm (where a weight is given) and rotation of q [tokens,
     q_heads, dim] and k [tokens, kv_heads, dim] into q_out and k_out (which may be
     q and k).  positions int32 [tokens]; a negative one leaves its token out."""
-    code, device = _act(q, "q"), q.get_device()
-    _here(device)
+    code, dtype, device = _act(q, "q"), q.dtype, q.get_device()
+    st = _launch_stream(device, stream)
     if q.dim() != 3 or k.dim() != 3:
         raise _bad("q and k must be [tokens, heads, dim]")
-    qh, kh, dim = q.shape[1], k.shape[1], q.shape[2]
-    a, b = _rows(q, qh, dim, code, device, "q"), _rows(k, kh, dim, code, device, "k")
-    c, d = _rows(q_out, qh, dim, code, device, "q_out"), _rows(k_out, kh, dim, code, device, "k_out")
-    n = _tokens_of(a, b, c, d)
+    n, qh, dim = q.shape
+    kh = k.shape[1]
+    qp, qs, _ = _rows(q, qh, dim, dtype, device, "q")
+    kp, ks, n1 = _rows(k, kh, dim, dtype, device, "k")
+    qop, qos, n2 = _rows(q_out, qh, dim, dtype, device, "q_out")
+    kop, kos, n3 = _rows(k_out, kh, dim, dtype, device, "k_out")
+    _same(n, n1, n2, n3)
     norm = _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device)
-    check(lib().tir_qk_norm_rope(a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1],
-                                 _ints(positions, n, device, "positions"), n, qh, kh, dim, code, C.addressof(norm),
-                                 _stream(stream)))
+    check(lib().tir_qk_norm_rope(qp, qs, kp, ks, qop, qos, kop, kos, _ints(positions, n, device, "positions"), n, qh, kh,
+                                 dim, code, C.addressof(norm), st))
 
 
 def qk_norm_rope_append(q, k, v, q_out, kv, seqs, positions, rope=None, q_weight=None, k_weight=None, eps=1e-5,
                         pairs="adjacent", stream=None):
     """qk_norm_rope with the keys, and the values as they are, written to the
     cache: token t to position positions[t] of table row seqs[t] (None: row t)."""
-    code, device, dim, kh = _act(q, "q"), kv.device, kv.dim, kv.kv_heads
-    _here(device)
+    code, dtype, device, dim, kh = _act(q, "q"), q.dtype, kv.device, kv.dim, kv.kv_heads
+    st = _launch_stream(device, stream)
     if q.dim() != 3:
         raise _bad("q must be [tokens, heads, dim]")
-    qh = q.shape[1]
-    a, b = _rows(q, qh, dim, code, device, "q"), _rows(k, kh, dim, code, device, "k")
-    c, d = _rows(v, kh, dim, code, device, "v"), _rows(q_out, qh, dim, code, device, "q_out")
-    n = _tokens_of(a, b, c, d)
+    n, qh, _ = q.shape
+    qp, qs, _ = _rows(q, qh, dim, dtype, device, "q")
+    kp, ks, n1 = _rows(k, kh, dim, dtype, device, "k")
+    vp, vs, n2 = _rows(v, kh, dim, dtype, device, "v")
+    qop, qos, n3 = _rows(q_out, qh, dim, dtype, device, "q_out")
+    _same(n, n1, n2, n3)
     norm = _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device)
-    check(lib().tir_qk_norm_rope_append(a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1], kv.ref,
-                                        _ints(seqs, n, device, "seqs"), _ints(positions, n, device, "positions"), n,
-                                        qh, code, C.addressof(norm), _stream(stream)))
+    check(lib().tir_qk_norm_rope_append(qp, qs, kp, ks, vp, vs, qop, qos, kv.ref, _ints(seqs, n, device, "seqs"),
+                                        _ints(positions, n, device, "positions"), n, qh, code, C.addressof(norm), st))
 
 
 def kv_append(kv, k, v, seqs, positions, stream=None):
     """Rows k, v [tokens, kv_heads, dim] to the cache, rounded or quantised."""
-    code, device = _act(k, "k"), kv.device
-    _here(device)
-    a = _rows(k, kv.kv_heads, kv.dim, code, device, "k")
-    b = _rows(v, kv.kv_heads, kv.dim, code, device, "v")
-    n = _tokens_of(a, b)
-    check(lib().tir_kv_append(kv.ref, a[0], a[1], b[0], b[1], _ints(seqs, n, device, "seqs"),
-                              _ints(positions, n, device, "positions"), n, code, _stream(stream)))
+    code, dtype, device = _act(k, "k"), k.dtype, kv.device
+    st = _launch_stream(device, stream)
+    kp, ks, n = _rows(k, kv.kv_heads, kv.dim, dtype, device, "k")
+    vp, vs, n1 = _rows(v, kv.kv_heads, kv.dim, dtype, device, "v")
+    _same(n, n1)
+    check(lib().tir_kv_append(kv.ref, kp, ks, vp, vs, _ints(seqs, n, device, "seqs"),
+                              _ints(positions, n, device, "positions"), n, code, st))
 
 
 def kv_gather(kv, k_out, v_out, seqs, positions, stream=None):
     """Cached positions back as rows k_out, v_out [tokens, kv_heads, dim]."""
-    code, device = _act(k_out, "k_out"), kv.device
-    _here(device)
-    a = _rows(k_out, kv.kv_heads, kv.dim, code, device, "k_out")
-    b = _rows(v_out, kv.kv_heads, kv.dim, code, device, "v_out")
-    n = _tokens_of(a, b)
-    check(lib().tir_kv_gather(kv.ref, a[0], a[1], b[0], b[1], _ints(seqs, n, device, "seqs"),
-                              _ints(positions, n, device, "positions"), n, code, _stream(stream)))
+    code, dtype, device = _act(k_out, "k_out"), k_out.dtype, kv.device
+    st = _launch_stream(device, stream)
+    kp, ks, n = _rows(k_out, kv.kv_heads, kv.dim, dtype, device, "k_out")
+    vp, vs, n1 = _rows(v_out, kv.kv_heads, kv.dim, dtype, device, "v_out")
+    _same(n, n1)
+    check(lib().tir_kv_gather(kv.ref, kp, ks, vp, vs, _ints(seqs, n, device, "seqs"),
+                              _ints(positions, n, device, "positions"), n, code, st))
 
 
 def paged_attention_workspace(kv, rows, q_heads, max_len=0, window=0):
@@ -1031,23 +1057,26 @@ def paged_attention(q, kv, seq_lens, out, scale=0.0, max_len=0, window=0, worksp
     zeros for a row of length 0.  workspace: a uint8 tensor of
     paged_attention_workspace bytes; without one it is taken from torch's allocator
     for the call, on the current stream."""
-    code, device = _act(q, "q"), kv.device
-    _here(device)
+    code, dtype, device = _act(q, "q"), q.dtype, kv.device
+    st = _launch_stream(device, stream)
     if q.dim() != 3:
         raise _bad("q must be [rows, q_heads, dim]")
-    qh = q.shape[1]
-    a, b = _rows(q, qh, kv.dim, code, device, "q"), _rows(out, qh, kv.dim, code, device, "out")
-    n = _tokens_of(a, b)
+    n, qh, _ = q.shape
+    qp, qs, _ = _rows(q, qh, kv.dim, dtype, device, "q")
+    op, os_, n1 = _rows(out, qh, kv.dim, dtype, device, "out")
+    _same(n, n1)
+    size = wp = 0
     if workspace is None:
         size = paged_attention_workspace(kv, n, qh, max_len, window)
         if size:
             import torch
-            if stream is not None and _stream(stream) != torch.cuda.current_stream().cuda_stream:
+            if st != _torch().stream(device):
                 raise _bad("paged_attention on another stream than the current one needs a workspace")
             workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-    elif workspace.get_device() != device or not workspace.is_contiguous():
-        raise _bad(f"workspace must be a contiguous tensor on device {device}")
-    check(lib().tir_paged_attention(a[0], a[1], kv.ref, _ints(seq_lens, n, device, "seq_lens"), b[0], b[1], n, qh,
-                                    code, scale, max_len, window, _ptr(workspace),
-                                    workspace.numel() * workspace.element_size() if workspace is not None else 0,
-                                    _stream(stream)))
+            wp = workspace.data_ptr()
+    else:
+        if workspace.get_device() != device or not workspace.is_contiguous():
+            raise _bad(f"workspace must be a contiguous tensor on device {device}")
+        size, wp = workspace.nbytes, workspace.data_ptr()
+    check(lib().tir_paged_attention(qp, qs, kv.ref, _ints(seq_lens, n, device, "seq_lens"), op, os_, n, qh, code, scale,
+                                    max_len, window, wp, size, st))
