@@ -95,16 +95,22 @@ __device__ __forceinline__ void expand_q8x4(uint32_t w, float step, float* f) {
     for (int i = 0; i < 4; ++i) f[i] = __fmul_rn(static_cast<float>(static_cast<int8_t>(w >> (8 * i))), step);
 }
 
-// Page lookup shared by the kernels: page id of `pos` in table row `row`, -1
-// (and the error bit) where it lies outside.
-__device__ __forceinline__ int32_t page_of(const PagesView& v, int64_t row, int32_t pos) {
+// Page lookup shared by the kernels: the id the table holds for `pos` of row
+// `row`, and whether it lies in the pool (else the error bit is set).
+__device__ __forceinline__ int32_t page_id(const PagesView& v, int64_t row, int32_t pos) {
     const int32_t i = v.page_shift >= 0 ? pos >> v.page_shift : pos / v.page_size;
-    const int32_t id = __ldg(v.table + row * v.table_stride + i);
-    if (static_cast<uint32_t>(id) >= static_cast<uint64_t>(v.n_pages)) {
-        atomicOr(v.err, kBadPage);
-        return -1;
-    }
-    return id;
+    return __ldg(v.table + row * v.table_stride + i);
+}
+
+__device__ __forceinline__ bool page_ok(const PagesView& v, int32_t id) {
+    if (static_cast<uint32_t>(id) < static_cast<uint32_t>(v.n_pages)) return true;
+    atomicOr(v.err, kBadPage);
+    return false;
+}
+
+__device__ __forceinline__ int32_t page_of(const PagesView& v, int64_t row, int32_t pos) {
+    const int32_t id = page_id(v, row, pos);
+    return page_ok(v, id) ? id : -1;
 }
 
 // Element offset of `pos` in page `id` (head 0).

@@ -52,8 +52,6 @@ struct AttnArgs {
     float *part_o, *part_ml;  // [rows][q_heads][splits][dim], [..][splits][2]
 };
 
-constexpr int kAttnTile = 16;  // positions of a warp's tile
-
 // The part of a row's positions that split `i` of `splits` takes, in units of
 // `unit` positions: as even as whole units allow, none below `min_units` units.
 // `used` splits have any.
@@ -83,8 +81,9 @@ __device__ __forceinline__ int32_t row_length(const AttnArgs& a, const PagesView
 }
 
 // ---- instruction wrappers ----------------------------------------------------
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+// Copies 16 bytes, or (size 0) writes zeros and reads nothing.
+__device__ __forceinline__ void cp_async16_sized(uint32_t dst, const void* src, int size) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
 }
 
 template <int B>
@@ -154,13 +153,42 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// Two int8 of `w` picked by `sel` (biased bytes) as exact f16 integers: the byte
-// 128 + n under the exponent of 1024 reads 1152 + n.
-__device__ __forceinline__ uint32_t q8_pair(uint32_t w_biased, uint32_t sel) {
-    const uint32_t x = __byte_perm(w_biased, 0x64646464u, sel);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&h);
+// Four int8 as exact f16 integers: bytes 0 and 2 in *even, 1 and 3 in *odd.  The
+// byte 128 + n under the exponent of 1024 reads 1152 + n.
+__device__ __forceinline__ void q8_pairs(uint32_t w, uint32_t* even, uint32_t* odd) {
+    const uint32_t a = (w & 0x00ff00ffu) ^ 0x64806480u, b = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+    *even = *reinterpret_cast<const uint32_t*>(&x);
+    *odd = *reinterpret_cast<const uint32_t*>(&y);
 }
+
+// The Q8_0 steps of one position's head: D / 32 halves in one load.
+template <int D>
+struct Steps {
+    uint32_t w[D / 64];
+    __device__ __forceinline__ void load(const uint8_t* p, int key) {
+        if constexpr (D == 64) {
+            w[0] = reinterpret_cast<const uint32_t*>(p)[key];
+        } else if constexpr (D == 128) {
+            const uint2 x = reinterpret_cast<const uint2*>(p)[key];
+            w[0] = x.x, w[1] = x.y;
+        } else {
+            const uint4 x = reinterpret_cast<const uint4*>(p)[key];
+            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        }
+    }
+    __device__ __forceinline__ float get(int b) const {
+        return __half2float(__ushort_as_half(static_cast<uint16_t>(b & 1 ? w[b / 2] >> 16 : w[b / 2] & 0xffffu)));
+    }
+    // the larger magnitudes of the even and the odd blocks, as two 16-bit patterns
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int i = 1; i < D / 64; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+        return m;
+    }
+};
 
 // ---- configuration -----------------------------------------------------------
 // C: cache type; D: head size; NT: tiles of 8 query heads a CTA takes; F32Q: f32
@@ -173,18 +201,25 @@ struct AttnCfg {
     static constexpr int NP = tf32 ? 2 : bf && F32Q ? 3 : 2;      // parts of p
     // f16 operands hold q under a per-head power of two, but for f16 queries of f16 caches (exact as they are)
     static constexpr bool scaled = q8 || (C == Elem::F16 && F32Q);
+    // f32 queries take the scores' factor in before they are split; unscaled ones
+    // leave nothing to multiply a score by
+    static constexpr bool plain = F32Q && !scaled;
     static constexpr int ROW = D * ES;
+    // positions of a warp's tile: 32 where rows are short, so that the work around a
+    // tile (pages, copies, votes) is shared by more of them
+    static constexpr int TILE = ROW <= 128 ? 32 : 16;
+    static constexpr int MT = TILE / 16;
     static constexpr int PITCH = ROW + 16;  // an odd number of 16-byte units: ldmatrix rows fall on different banks
     static constexpr int STEPS = q8 ? D / 32 * 2 : 0;  // bytes of a position's Q8_0 steps
-    static constexpr int V_AT = kAttnTile * PITCH;
-    static constexpr int KS_AT = 2 * kAttnTile * PITCH, VS_AT = KS_AT + kAttnTile * STEPS;
-    static constexpr int STAGE = KS_AT + 2 * kAttnTile * STEPS;
+    static constexpr int V_AT = TILE * PITCH;
+    static constexpr int KS_AT = 2 * TILE * PITCH, VS_AT = KS_AT + TILE * STEPS;
+    static constexpr int STAGE = KS_AT + 2 * TILE * STEPS;
     static constexpr int KSTEPS = tf32 ? D / 8 : D / 16;  // q operand steps
     static constexpr int QBYTES = KSTEPS * NT * NQ * 256;
     static constexpr int HEADS = 8 * NT;
     static constexpr int WARPS = STAGE > 32 * 1024 ? 2 : 4;
     static constexpr int THREADS = WARPS * 32;
-    static constexpr int UNIT = WARPS * kAttnTile;
+    static constexpr int UNIT = WARPS * TILE;
     static constexpr int FIXED = QBYTES + HEADS * 4 + WARPS * HEADS * 8;
     // two CTAs an SM where three stages fit in half of its shared memory, else one
     static constexpr int half_stages = (112 * 1024 - FIXED) / (WARPS * STAGE);
@@ -206,7 +241,8 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     paged_attn_kernel(const AttnArgs a, const PagesView kv) {
     using X = AttnCfg<C, D, NT, F32Q>;
     constexpr uint32_t FULL = 0xffffffffu;
-    constexpr int CH = X::ROW / 16;  // 16-byte pieces of a cached row
+    constexpr int CH = X::ROW / 16;        // 16-byte pieces of a cached row
+    constexpr int LPR = CH < 8 ? CH : 8;  // lanes that copy a row
     // weights are kept 2^6 above their logarithm's reference, and the reference may
     // lag the maximum by 8: f16 parts then lose nothing to the end of its range
     constexpr float kLift = X::tf32 || X::bf ? 0.f : 6.f;
@@ -243,41 +279,51 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     if (range.k0 >= range.k1) return;
 
     // ---- the ring ----
-    const int n_tiles = (range.k1 - range.k0 + kAttnTile - 1) / kAttnTile;
+    const int n_tiles = (range.k1 - range.k0 + X::TILE - 1) / X::TILE;
     const int my_tiles = n_tiles > warp ? (n_tiles - warp + X::WARPS - 1) / X::WARPS : 0;
     uint8_t* my_ring = ring + warp * X::STAGES * X::STAGE;
     const uint32_t ring_addr = smem_u32(my_ring);
-    // page of this lane's position (lane % 16) of the warp's tile i; -1 past the end
+    // this lane's position (lane % TILE) of the warp's tile i, and the page it is on:
+    // asked for one tile before its copies are issued, checked only then
+    auto position = [&](int i) -> int32_t { return range.k0 + (i * X::WARPS + warp) * X::TILE + (lane & (X::TILE - 1)); };
     auto lookup = [&](int i) -> int32_t {
-        const int32_t pos = range.k0 + (i * X::WARPS + warp) * kAttnTile + (lane & 15);
-        return i < my_tiles && pos < range.k1 ? page_of(kv, row, pos) : -1;
+        const int32_t pos = position(i);
+        return pos < range.k1 ? page_id(kv, row, pos) : -1;
     };
     const int64_t head_at = static_cast<int64_t>(hk) * kv.head_stride;
-    auto issue = [&](int i, int32_t page) {
+    const int64_t k_to_v = kv.v - kv.k;
+    auto issue = [&](int i, int slot, int32_t page) {
         if (i < my_tiles) {
-            const int32_t pos = range.k0 + (i * X::WARPS + warp) * kAttnTile + (lane & 15);
-            const int64_t mine = page < 0 ? -1 : slot_of(kv, page, pos) + head_at;
-            const uint32_t dst = ring_addr + (i % X::STAGES) * X::STAGE;
+            const int32_t pos = position(i);
+            int64_t mine = -1;
+            if (pos < range.k1 && page_ok(kv, page)) mine = slot_of(kv, page, pos) + head_at;
+            const uint32_t dst = ring_addr + slot * X::STAGE;
             if constexpr (X::q8) {
                 const bool live = mine >= 0;
-                const uint16_t* src = (lane < 16 ? kv.ks : kv.vs) + (live ? mine >> 5 : 0);
-                cp_async_small_or_zero<X::STEPS>(dst + (lane < 16 ? X::KS_AT : X::VS_AT) + (lane & 15) * X::STEPS, src, live);
+                const int64_t at = live ? mine >> 5 : 0;
+                const uint32_t to = dst + (lane & (X::TILE - 1)) * X::STEPS;
+                if (X::TILE == 32 || lane < 16) cp_async_small_or_zero<X::STEPS>(to + X::KS_AT, kv.ks + at, live);
+                if (X::TILE == 32 || lane >= 16) cp_async_small_or_zero<X::STEPS>(to + X::VS_AT, kv.vs + at, live);
             }
+            // a 128-byte line (or a whole shorter row) at a time
 #pragma unroll
-            for (int u = 0; u < kAttnTile * CH / 32; ++u) {
-                const int idx = u * 32 + lane, key = idx / CH, ch = idx % CH;
+            for (int u = 0; u < X::TILE * LPR / 32; ++u) {
+                const int key = u * (32 / LPR) + lane / LPR;
                 const int64_t at = __shfl_sync(FULL, mine, key);
-                const bool live = at >= 0;
-                const int64_t byte = (live ? at : 0) * X::ES + ch * 16;
-                const uint32_t to = dst + key * X::PITCH + ch * 16;
-                cp_async16_or_zero(to, kv.k + (live ? byte : 0), live);
-                cp_async16_or_zero(to + X::V_AT, kv.v + (live ? byte : 0), live);
+                const int size = at >= 0 ? 16 : 0;
+                const char* from = kv.k + (at >= 0 ? at * X::ES : 0) + (lane % LPR) * 16;
+                const uint32_t to = dst + key * X::PITCH + (lane % LPR) * 16;
+#pragma unroll
+                for (int ch = 0; ch < CH; ch += LPR) {
+                    cp_async16_sized(to + ch * 16, from + ch * 16, size);
+                    cp_async16_sized(to + X::V_AT + ch * 16, from + k_to_v + ch * 16, size);
+                }
             }
         }
         cp_async_commit();
     };
 #pragma unroll
-    for (int i = 0; i < X::STAGES - 1; ++i) issue(i, lookup(i));
+    for (int i = 0; i < X::STAGES - 1; ++i) issue(i, i, lookup(i));
     int32_t next_page = lookup(X::STAGES - 1);
 
     // ---- q operands, while the first tiles are on their way ----
@@ -293,22 +339,23 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                        : a.act == Elem::F16 ? __half2float(reinterpret_cast<const __half*>(a.q)[at])
                                             : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.q)[at]);
             }
+            if constexpr (F32Q) x[i] *= a.scale_log2;
             top = fmaxf(top, fabsf(x[i]));
         }
-        float c = a.scale_log2;
+        float c = F32Q ? 1.f : a.scale_log2;
         if constexpr (X::scaled) {
 #pragma unroll
             for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
             const int e = static_cast<int>(__float_as_uint(top) >> 23);  // biased exponent
             if (e > 0 && e < 255) {                                      // top * 2^s in [2^9, 2^10)
-                const int s = min(136 - e, 120);
+                const int s = min(136 - e, 60);  // below 2^-51 every score rounds to 0 whatever its digits
                 const float up = __uint_as_float(static_cast<uint32_t>(127 + s) << 23);
                 c *= __uint_as_float(static_cast<uint32_t>(127 - s) << 23);
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) x[i] *= up;
             }
         }
-        if (lane == 0) cs[j] = c;
+        if (lane == 0) cs[j] = fmaxf(c, 1.2e-38f);  // never 0: a masked score is c * -inf
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
             const int e = i * 32 + lane;  // element of the head
@@ -317,14 +364,14 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                 split_tf32(x[i], &qf[at], &qf[at + 64]);
             } else {
                 // operand element k = 2 t' + {0, 1} (+ 8 in the second register); Q8_0 words
-                // hold elements 4 t' .. 4 t' + 3, so there the order inside 16 is theirs
+                // hold elements 4 t' .. 4 t' + 3 and give bytes 0, 2 and 1, 3: there the order is theirs
                 const int kk = e / 16, r = e % 16;
-                const int tt = X::q8 ? r / 4 : r % 8 / 2, reg = X::q8 ? r % 4 / 2 : r / 8;
+                const int tt = X::q8 ? r / 4 : r % 8 / 2, reg = X::q8 ? r & 1 : r / 8;
                 float rem = x[i];
 #pragma unroll
                 for (int s = 0; s < X::NQ; ++s) {
                     const int at = (((kk * NT + j / 8) * X::NQ + s) * 32 + (j % 8) * 4 + tt) * 2 + reg;
-                    uint16_t* p = reinterpret_cast<uint16_t*>(qf + at) + (r & 1);
+                    uint16_t* p = reinterpret_cast<uint16_t*>(qf + at) + (X::q8 ? r % 4 / 2 : r & 1);
                     if constexpr (X::bf) {
                         const __nv_bfloat16 b = __float2bfloat16_rn(rem);
                         *p = __bfloat16_as_ushort(b);
@@ -353,13 +400,14 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         if constexpr (X::q_in_regs) return make_uint2(qr[2 * i], qr[2 * i + 1]);
         else return reinterpret_cast<const uint2*>(qf)[i * 32 + lane];
     };
-    float c[NT][2], m[NT][2], l[NT][2], o[D / 16][NT][4];
+    float c[NT][2], m[NT][2], base[NT][2], l[NT][2], o[D / 16][NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             c[n][e] = cs[n * 8 + 2 * t + e];
             m[n][e] = -INFINITY;
+            base[n][e] = -kLift;
             l[n][e] = 0.f;
         }
 #pragma unroll
@@ -370,134 +418,144 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
             for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
     int v_exp = 0;  // Q8_0: o is kept over 2^(v_exp - 14), the power of two above the steps seen so far
 
+    // c s - base.  The product is rounded (or exact: c is a power of two under f32
+    // queries) before the difference is taken, as the maximum's was: equal scores
+    // stay equal whatever their size.
+    auto above = [&](float s, int n, int e) -> float {
+        if constexpr (X::plain) return s - base[n][e];
+        else if constexpr (F32Q) return fmaf(s, c[n][e], -base[n][e]);
+        else return __fadd_rn(__fmul_rn(s, c[n][e]), -base[n][e]);
+    };
+
     // ---- the loop over this warp's tiles ----
+    int slot = 0, free_slot = X::STAGES - 1;
     for (int it = 0; it < my_tiles; ++it) {
         cp_async_wait<X::STAGES - 2>();
         __syncwarp();
-        issue(it + X::STAGES - 1, next_page);
+        issue(it + X::STAGES - 1, free_slot, next_page);
         next_page = lookup(it + X::STAGES);
-        const uint8_t* st = my_ring + (it % X::STAGES) * X::STAGE;
-        const uint32_t sa = ring_addr + (it % X::STAGES) * X::STAGE;
+        const uint8_t* st = my_ring + slot * X::STAGE;
+        const uint32_t sa = ring_addr + slot * X::STAGE;
+        free_slot = slot;
+        slot = slot + 1 == X::STAGES ? 0 : slot + 1;
         const uint32_t row_addr = sa + (lane & 15) * X::PITCH + (lane >> 4) * 16;
 
         // S' = K Q'
-        float s[NT][4];
+        float s[X::MT][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int mt = 0; mt < X::MT; ++mt) {
+            const uint32_t k_addr = row_addr + mt * 16 * X::PITCH;
+            float s2[NT][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-        if constexpr (X::q8) {
-            uint16_t k_steps[2][D / 32];
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+                for (int e = 0; e < 4; ++e) s[mt][n][e] = s2[n][e] = 0.f;
+            if constexpr (X::q8) {
+                Steps<D> k_steps[2];
+                k_steps[0].load(st + X::KS_AT, mt * 16 + g);
+                k_steps[1].load(st + X::KS_AT, mt * 16 + g + 8);
 #pragma unroll
-                for (int b = 0; b < D / 32; ++b)
-                    k_steps[half][b] = reinterpret_cast<const uint16_t*>(st + X::KS_AT)[(g + 8 * half) * (D / 32) + b];
+                for (int b = 0; b < D / 32; ++b) {
+                    uint32_t w[4], x0[4], x1[4];
+                    ldsm4(w, k_addr + b * 32);
+                    q8_pairs(w[0], &x0[0], &x0[2]);
+                    q8_pairs(w[1], &x0[1], &x0[3]);
+                    q8_pairs(w[2], &x1[0], &x1[2]);
+                    q8_pairs(w[3], &x1[1], &x1[3]);
+                    const float d0 = k_steps[0].get(b), d1 = k_steps[1].get(b);
 #pragma unroll
-            for (int b = 0; b < D / 32; ++b) {
-                uint32_t w[4], x0[4], x1[4];
-                ldsm4(w, row_addr + b * 32);
+                    for (int n = 0; n < NT; ++n) {
+                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
-                x0[0] = q8_pair(w[0], 0x4140), x0[1] = q8_pair(w[1], 0x4140);
-                x0[2] = q8_pair(w[0], 0x4342), x0[3] = q8_pair(w[1], 0x4342);
-                x1[0] = q8_pair(w[2], 0x4140), x1[1] = q8_pair(w[3], 0x4140);
-                x1[2] = q8_pair(w[2], 0x4342), x1[3] = q8_pair(w[3], 0x4342);
-                const float d0 = __half2float(__ushort_as_half(k_steps[0][b])), d1 = __half2float(__ushort_as_half(k_steps[1][b]));
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int p = X::NQ - 1; p >= 0; --p) {
-                        const uint2 q0 = q_op(2 * b, n, p), q1 = q_op(2 * b + 1, n, p);
-                        mma16<false>(acc, x0, q0.x, q0.y);
-                        mma16<false>(acc, x1, q1.x, q1.y);
+                        for (int p = X::NQ - 1; p >= 0; --p) {
+                            const uint2 q0 = q_op(2 * b, n, p), q1 = q_op(2 * b + 1, n, p);
+                            mma16<false>(acc, x0, q0.x, q0.y);
+                            mma16<false>(acc, x1, q1.x, q1.y);
+                        }
+                        s[mt][n][0] = fmaf(acc[0], d0, s[mt][n][0]);
+                        s[mt][n][1] = fmaf(acc[1], d0, s[mt][n][1]);
+                        s[mt][n][2] = fmaf(acc[2], d1, s[mt][n][2]);
+                        s[mt][n][3] = fmaf(acc[3], d1, s[mt][n][3]);
                     }
-                    s[n][0] = fmaf(acc[0], d0, s[n][0]);
-                    s[n][1] = fmaf(acc[1], d0, s[n][1]);
-                    s[n][2] = fmaf(acc[2], d1, s[n][2]);
-                    s[n][3] = fmaf(acc[3], d1, s[n][3]);
+                }
+            } else if constexpr (X::tf32) {
+#pragma unroll
+                for (int kk = 0; kk < D / 8; ++kk) {
+                    uint32_t w[4], hi[4], lo[4];
+                    ldsm4(w, k_addr + kk * 32);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split_tf32(__uint_as_float(w[e]), &hi[e], &lo[e]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const uint2 qh = q_op(kk, n, 0), ql = q_op(kk, n, 1);
+                        mma8(s2[n], lo, qh.x, qh.y);
+                        mma8(s2[n], hi, ql.x, ql.y);
+                        mma8(s[mt][n], hi, qh.x, qh.y);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    uint32_t w[4];
+                    ldsm4(w, k_addr + kk * 32);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int p = X::NQ - 1; p >= 0; --p) {
+                            const uint2 qv = q_op(kk, n, p);
+                            mma16<X::bf>(((kk + p) & 1) ? s2[n] : s[mt][n], w, qv.x, qv.y);
+                        }
                 }
             }
-        } else if constexpr (X::tf32) {
-            float s2[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s2[n][e] = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < D / 8; ++kk) {
-                uint32_t w[4], hi[4], lo[4];
-                ldsm4(w, row_addr + kk * 32);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) split_tf32(__uint_as_float(w[e]), &hi[e], &lo[e]);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const uint2 qh = q_op(kk, n, 0), ql = q_op(kk, n, 1);
-                    mma8(s2[n], lo, qh.x, qh.y);
-                    mma8(s2[n], hi, ql.x, ql.y);
-                    mma8(s[n], hi, qh.x, qh.y);
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
-        } else {
-            float s2[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s2[n][e] = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                uint32_t w[4];
-                ldsm4(w, row_addr + kk * 32);
+            if constexpr (!X::q8) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int p = X::NQ - 1; p >= 0; --p) {
-                        const uint2 qv = q_op(kk, n, p);
-                        mma16<X::bf>(((kk + p) & 1) ? s2[n] : s[n], w, qv.x, qv.y);
-                    }
+                    for (int e = 0; e < 4; ++e) s[mt][n][e] += s2[n][e];
             }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
         }
 
         // weights: p = 2^(t - m + lift), with m moved only when a score passes it by
         // more than kLag (rare after the first tiles): no reduction in the usual tile
-        const int32_t key0 = range.k0 + (it * X::WARPS + warp) * kAttnTile + g;
+        const int32_t left = range.k1 - (range.k0 + (it * X::WARPS + warp) * X::TILE);  // positions of this tile
+        if (left < X::TILE) {
+#pragma unroll
+            for (int mt = 0; mt < X::MT; ++mt)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (mt * 16 + g + (e >> 1) * 8 >= left) s[mt][n][e] = -INFINITY;
+        }
         bool moves = false;
         float top[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                s[n][e] = key0 < range.k1 ? s[n][e] * c[n][e] : -INFINITY;
-                s[n][e + 2] = key0 + 8 < range.k1 ? s[n][e + 2] * c[n][e] : -INFINITY;
-                top[n][e] = fmaxf(s[n][e], s[n][e + 2]);
+                top[n][e] = fmaxf(s[0][n][e], s[0][n][e + 2]);
+#pragma unroll
+                for (int mt = 1; mt < X::MT; ++mt) top[n][e] = fmaxf(top[n][e], fmaxf(s[mt][n][e], s[mt][n][e + 2]));
+                if constexpr (!X::plain) top[n][e] *= c[n][e];
                 moves |= top[n][e] > m[n][e] + kLag;
             }
+        Steps<X::q8 ? D : 64> v_steps[X::MT][2];
         uint32_t v_top = 0u;
-        uint16_t v_steps[2][X::q8 ? D / 32 : 1];
         if constexpr (X::q8) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int mt = 0; mt < X::MT; ++mt)
 #pragma unroll
-                for (int b = 0; b < D / 32; ++b) {
-                    v_steps[half][b] = reinterpret_cast<const uint16_t*>(st + X::VS_AT)[(g + 8 * half) * (D / 32) + b];
-                    v_top = max(v_top, static_cast<uint32_t>(v_steps[half][b] & 0x7fffu) >> 10);
+                for (int half = 0; half < 2; ++half) {
+                    v_steps[mt][half].load(st + X::VS_AT, mt * 16 + g + 8 * half);
+                    v_top = __vmaxu2(v_top, v_steps[mt][half].top());
                 }
+            v_top = max(v_top & 0xffffu, v_top >> 16) >> 10;
             moves |= static_cast<int>(v_top) > v_exp;
         }
         if (__any_sync(FULL, moves)) {
             float shrink = 1.f;
             if constexpr (X::q8) {
-#pragma unroll
-                for (int w = 16; w; w >>= 1) v_top = max(v_top, __shfl_xor_sync(FULL, v_top, w));
+                v_top = __reduce_max_sync(FULL, v_top);
                 const int up = max(static_cast<int>(v_top) - v_exp, 0);
                 shrink = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
                 v_exp += up;
@@ -512,6 +570,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                     const float mn = fmaxf(m[n][e], top[n][e]);
                     const float corr = m[n][e] == mn ? 1.f : exp2_fast(m[n][e] - mn);
                     m[n][e] = mn;
+                    base[n][e] = (mn == -INFINITY ? 0.f : mn) - kLift;
                     l[n][e] *= corr;
                     f[e] = corr * shrink;
                 }
@@ -525,101 +584,103 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
             }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int mt = 0; mt < X::MT; ++mt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float base = (m[n][e] == -INFINITY ? 0.f : m[n][e]) - kLift;
-                s[n][e] = exp2_fast(s[n][e] - base);
-                s[n][e + 2] = exp2_fast(s[n][e + 2] - base);
-                l[n][e] += s[n][e] + s[n][e + 2];
-            }
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    s[mt][n][e] = exp2_fast(above(s[mt][n][e], n, e));
+                    s[mt][n][e + 2] = exp2_fast(above(s[mt][n][e + 2], n, e));
+                    l[n][e] += s[mt][n][e] + s[mt][n][e + 2];
+                }
 
         // O' += V' P'
-        if constexpr (X::q8) {
-            const float inv = __uint_as_float(static_cast<uint32_t>(127 + 14 - v_exp) << 23);
 #pragma unroll
-            for (int b = 0; b < D / 32; ++b) {
-                const float d0 = __half2float(__ushort_as_half(v_steps[0][b])) * inv;
-                const float d1 = __half2float(__ushort_as_half(v_steps[1][b])) * inv;
-                uint32_t p0[NT][2], p1[NT][2];
+        for (int mt = 0; mt < X::MT; ++mt) {
+            if constexpr (X::q8) {
+                const float inv = __uint_as_float(static_cast<uint32_t>(127 + 14 - v_exp) << 23);
+                const uint32_t v_addr = row_addr + X::V_AT + mt * 16 * X::PITCH;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float w0 = s[n][0] * d0, w1 = s[n][1] * d0, w2 = s[n][2] * d1, w3 = s[n][3] * d1;
-                    const __half2 ha = __floats2half2_rn(w0, w1), hb = __floats2half2_rn(w2, w3);
-                    const float2 fa = __half22float2(ha), fb = __half22float2(hb);
-                    p0[n][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&ha));
-                    p0[n][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hb));
-                    p1[n][0] = transpose8x8(pack2(w0 - fa.x, w1 - fa.y, Elem::F16));
-                    p1[n][1] = transpose8x8(pack2(w2 - fb.x, w3 - fb.y, Elem::F16));
-                }
-                uint32_t w[4];
-                ldsm4_t(w, sa + X::V_AT + (lane & 15) * X::PITCH + b * 32 + (lane >> 4) * 16);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t x[4];
-                    x[0] = q8_pair(w[2 * i], 0x4240), x[1] = q8_pair(w[2 * i], 0x4341);
-                    x[2] = q8_pair(w[2 * i + 1], 0x4240), x[3] = q8_pair(w[2 * i + 1], 0x4341);
+                for (int b = 0; b < D / 32; ++b) {
+                    const float d0 = v_steps[mt][0].get(b) * inv, d1 = v_steps[mt][1].get(b) * inv;
+                    uint32_t p0[NT][2], p1[NT][2];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        mma16<false>(o[2 * b + i][n], x, p1[n][0], p1[n][1]);
-                        mma16<false>(o[2 * b + i][n], x, p0[n][0], p0[n][1]);
+                        const float w0 = s[mt][n][0] * d0, w1 = s[mt][n][1] * d0, w2 = s[mt][n][2] * d1, w3 = s[mt][n][3] * d1;
+                        const __half2 ha = __floats2half2_rn(w0, w1), hb = __floats2half2_rn(w2, w3);
+                        const float2 fa = __half22float2(ha), fb = __half22float2(hb);
+                        p0[n][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&ha));
+                        p0[n][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hb));
+                        p1[n][0] = transpose8x8(pack2(w0 - fa.x, w1 - fa.y, Elem::F16));
+                        p1[n][1] = transpose8x8(pack2(w2 - fb.x, w3 - fb.y, Elem::F16));
+                    }
+                    uint32_t w[4];
+                    ldsm4_t(w, v_addr + b * 32);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t x[4];
+                        q8_pairs(w[2 * i], &x[0], &x[1]);
+                        q8_pairs(w[2 * i + 1], &x[2], &x[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma16<false>(o[2 * b + i][n], x, p1[n][0], p1[n][1]);
+                            mma16<false>(o[2 * b + i][n], x, p0[n][0], p0[n][1]);
+                        }
                     }
                 }
-            }
-        } else if constexpr (X::tf32) {
+            } else if constexpr (X::tf32) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                uint32_t ph[NT][2], pl[NT][2];
+                for (int kb = 0; kb < 2; ++kb) {
+                    uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const uint32_t x = __float_as_uint(s[mt][n][2 * kb]), y = __float_as_uint(s[mt][n][2 * kb + 1]);
+                        const uint32_t up = transpose8x8(__byte_perm(x, y, 0x7632)), dn = transpose8x8(__byte_perm(x, y, 0x5410));
+                        split_tf32(__uint_as_float(__byte_perm(dn, up, 0x5410)), &ph[n][0], &pl[n][0]);
+                        split_tf32(__uint_as_float(__byte_perm(dn, up, 0x7632)), &ph[n][1], &pl[n][1]);
+                    }
+                    const uint8_t* v = st + X::V_AT + (mt * 16 + 8 * kb + 2 * t) * X::PITCH + g * 8;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const float2 va = *reinterpret_cast<const float2*>(v + i * 64);
+                        const float2 vb = *reinterpret_cast<const float2*>(v + X::PITCH + i * 64);
+                        uint32_t hi[4], lo[4];
+                        split_tf32(va.x, &hi[0], &lo[0]);
+                        split_tf32(va.y, &hi[1], &lo[1]);
+                        split_tf32(vb.x, &hi[2], &lo[2]);
+                        split_tf32(vb.y, &hi[3], &lo[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma8(o[i][n], lo, ph[n][0], ph[n][1]);
+                            mma8(o[i][n], hi, pl[n][0], pl[n][1]);
+                            mma8(o[i][n], hi, ph[n][0], ph[n][1]);
+                        }
+                    }
+                }
+            } else {
+                uint32_t pp[NT][X::NP][2];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const uint32_t x = __float_as_uint(s[n][2 * kb]), y = __float_as_uint(s[n][2 * kb + 1]);
-                    const uint32_t up = transpose8x8(__byte_perm(x, y, 0x7632)), dn = transpose8x8(__byte_perm(x, y, 0x5410));
-                    split_tf32(__uint_as_float(__byte_perm(dn, up, 0x5410)), &ph[n][0], &pl[n][0]);
-                    split_tf32(__uint_as_float(__byte_perm(dn, up, 0x7632)), &ph[n][1], &pl[n][1]);
+                    float r0 = s[mt][n][0], r1 = s[mt][n][1], r2 = s[mt][n][2], r3 = s[mt][n][3];
+#pragma unroll
+                    for (int p = 0; p < X::NP; ++p) {
+                        const uint32_t wa = pack2(r0, r1, C), wb = pack2(r2, r3, C);
+                        pp[n][p][0] = transpose8x8(wa);
+                        pp[n][p][1] = transpose8x8(wb);
+                        const float2 fa = unpack2(wa, C), fb = unpack2(wb, C);
+                        r0 -= fa.x, r1 -= fa.y, r2 -= fb.x, r3 -= fb.y;
+                    }
                 }
-                const uint8_t* v = st + X::V_AT + (8 * kb + 2 * t) * X::PITCH + g * 8;
+                const uint32_t v_addr = sa + X::V_AT + (mt * 16 + (lane & 7) + (lane >> 4) * 8) * X::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
-                    const float2 va = *reinterpret_cast<const float2*>(v + i * 64);
-                    const float2 vb = *reinterpret_cast<const float2*>(v + X::PITCH + i * 64);
-                    uint32_t hi[4], lo[4];
-                    split_tf32(va.x, &hi[0], &lo[0]);
-                    split_tf32(va.y, &hi[1], &lo[1]);
-                    split_tf32(vb.x, &hi[2], &lo[2]);
-                    split_tf32(vb.y, &hi[3], &lo[3]);
+                    uint32_t w[4];
+                    ldsm4_t(w, v_addr + i * 32);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma8(o[i][n], lo, ph[n][0], ph[n][1]);
-                        mma8(o[i][n], hi, pl[n][0], pl[n][1]);
-                        mma8(o[i][n], hi, ph[n][0], ph[n][1]);
-                    }
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int p = X::NP - 1; p >= 0; --p) mma16<X::bf>(o[i][n], w, pp[n][p][0], pp[n][p][1]);
                 }
-            }
-        } else {
-            uint32_t pp[NT][X::NP][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float r0 = s[n][0], r1 = s[n][1], r2 = s[n][2], r3 = s[n][3];
-#pragma unroll
-                for (int p = 0; p < X::NP; ++p) {
-                    const uint32_t wa = pack2(r0, r1, C), wb = pack2(r2, r3, C);
-                    pp[n][p][0] = transpose8x8(wa);
-                    pp[n][p][1] = transpose8x8(wb);
-                    const float2 fa = unpack2(wa, C), fb = unpack2(wb, C);
-                    r0 -= fa.x, r1 -= fa.y, r2 -= fb.x, r3 -= fb.y;
-                }
-            }
-            const uint32_t v_addr = sa + X::V_AT + ((lane & 7) + (lane >> 4) * 8) * X::PITCH + ((lane >> 3) & 1) * 16;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                uint32_t w[4];
-                ldsm4_t(w, v_addr + i * 32);
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int p = X::NP - 1; p >= 0; --p) mma16<X::bf>(o[i][n], w, pp[n][p][0], pp[n][p][1]);
             }
         }
     }

@@ -327,8 +327,8 @@ tir_status pages_view(const tir_kv_pages* kv, const char* entry, PagesView* v, E
     if (kv->kv_heads <= 0 || kv->page_size <= 0 || kv->max_pages <= 0 || kv->table_rows < 0 ||
         kv->table_stride < kv->max_pages || kv->n_pages <= 0 || kv->n_pages > INT32_MAX)
         return fail(TIR_ERR_INVALID_ARG, who + ": bad cache sizes");
-    if (static_cast<int64_t>(kv->max_pages) * kv->page_size > INT32_MAX)
-        return fail(TIR_ERR_UNSUPPORTED_SHAPE, who + ": a table row holds more than 2^31 - 1 positions");
+    if (static_cast<int64_t>(kv->max_pages) * kv->page_size > (1 << 30))
+        return fail(TIR_ERR_UNSUPPORTED_SHAPE, who + ": a table row holds more than 2^30 positions");
     const int64_t unit = q8 ? kv->dim : 16 / elem_bytes(*type);
     const int64_t strides[3] = {kv->page_stride, kv->pos_stride, kv->head_stride};
     for (int64_t s : strides)
