@@ -422,8 +422,10 @@ enum { TIR_DTYPE_F16 = 1, TIR_DTYPE_BF16 = 30 };
  * hold the int8 quants and k_scale / v_scale the f16 steps, that of the block
  * at element offset e at index e / 32.  `table` holds, per sequence, the pages
  * of its positions in order: position p is slot p % page_size of page
- * table[row * table_stride + p / page_size].  dim is 64, 128 or 256; pools are
- * 16-byte aligned, strides multiples of 16 bytes (Q8_0: of dim). */
+ * table[row * table_stride + p / page_size].  A row holds at most 2^30 positions, a
+ * pool spans less than 64 GB.
+ * dim is 64, 128 or 256; pools are 16-byte aligned, strides multiples of 16
+ * bytes (Q8_0: of dim). */
 typedef struct tir_kv_pages {
     void *k, *v;
     uint16_t *k_scale, *v_scale;  /* Q8_0 only */

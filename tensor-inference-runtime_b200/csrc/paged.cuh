@@ -119,4 +119,10 @@ __device__ __forceinline__ int64_t slot_of(const PagesView& v, int32_t id, int32
     return id * v.page_stride + in * v.pos_stride;
 }
 
+// The same in 16-byte units (a pool spans at most 2^32 of them).
+__device__ __forceinline__ uint32_t slot16_of(const PagesView& v, int32_t id, int32_t pos) {
+    const uint32_t in = v.page_shift >= 0 ? pos & (v.page_size - 1) : pos % v.page_size;
+    return id * v.page16 + in * v.pos16;
+}
+
 }  // namespace tir

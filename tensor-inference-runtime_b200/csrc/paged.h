@@ -24,6 +24,7 @@ struct PagesView {
     int64_t page_stride, pos_stride, head_stride;
     int32_t max_pages, page_size, page_shift;  // shift: log2(page_size), -1 where it is no power of two
     int32_t kv_heads, dim;
+    uint32_t page16, pos16, head16;  // the strides of the pools in 16-byte units
     uint32_t* err;  // sticky bits, kBad*
 };
 

@@ -102,8 +102,29 @@ struct Plan {
     int32_t splits, min_units;
 };
 
-// How many CTAs share a row: enough to fill the GPU twice over, and parts of at
-// most 32 units, so that rows of unequal length even out; none below two units.
+// How many CTAs share a row's head (s).  The time of a call is estimated for rows
+// that are all of the longest length,
+//   waves of (start + a part's units) + join,
+// and for rows spread evenly below it,
+//   all units over the GPU + starts + half a longest part + join,
+// and the s with the least sum of both is taken.  A unit costs a lone CTA kLone,
+// and an SM that holds several of them the time their bytes take (Q8_0: half as
+// much again, its conversions are the bound).  Constants measured on B200:
+// 64 rows x 4 heads x 2048 positions in f32 take 52 us with s = 1, 67 with 2 (a
+// second wave), 59 with 4; 64 rows x 8 heads up to 8192 in bf16 193 us with 1, 171
+// with 4, 205 with 16; one row of 131071 in bf16 1345 us with 1, 91 with 24.
+constexpr double kStart = 3.0, kLone = 0.9, kJoin = 1.5, kJoinRow = 1.0 / 1200.0;  // us
+constexpr double kBytesPerUs = 6.2e6;
+
+double split_time(int64_t items, int64_t units, int64_t s, int64_t slots, double unit_sm, int sms, int64_t heads) {
+    const int64_t per = (units + s - 1) / s, parts = (units + per - 1) / per, n = items * parts;
+    auto wave = [&](int64_t ctas) { return kStart + per * std::max(kLone, unit_sm * static_cast<double>(ctas) / sms); };
+    double even = static_cast<double>(n / slots) * wave(slots);
+    if (n % slots) even += wave(n % slots);
+    const double ragged = 0.5 * items * units * unit_sm / sms + kStart * 0.5 * items * (parts + 1) / slots + 0.5 * per * kLone;
+    return even + ragged + (parts > 1 ? 2 * (kJoin + kJoinRow * heads) : 0.0);
+}
+
 tir_status make_plan(const PagesView& kv, Elem cache, bool f32q, int64_t rows, int32_t q_heads, int64_t max_len,
                      int64_t window, Plan* p) {
     const int group = q_heads / kv.kv_heads;
@@ -116,14 +137,24 @@ tir_status make_plan(const PagesView& kv, Elem cache, bool f32q, int64_t rows, i
     if (max_len > 0) n = std::min(n, max_len);
     if (window > 0) n = std::min(n, window);
     const int64_t units = (n + p->shape.unit - 1) / p->shape.unit;
-    const int64_t base = std::max<int64_t>(rows * kv.kv_heads * p->head_tiles, 1);
+    const int64_t items = std::max<int64_t>(rows * kv.kv_heads * p->head_tiles, 1);
     const int64_t slots = static_cast<int64_t>(sms) * p->shape.per_sm;
-    p->min_units = 2;
-    int64_t splits = std::max((2 * slots + base - 1) / base, (units + 31) / 32);
-    splits = std::min(splits, (units + p->min_units - 1) / p->min_units);
-    splits = std::max<int64_t>(splits, 1);
-    if (base * splits > INT32_MAX) return fail(TIR_ERR_UNSUPPORTED_SHAPE, "tir_paged_attention: too many rows");
-    p->splits = static_cast<int32_t>(splits);
+    const double unit_sm = p->shape.unit * kv.dim * 2.0 * p->shape.bytes * sms / kBytesPerUs;
+    int64_t best = 1;
+    double least = 1e30;
+    auto consider = [&](int64_t s) {
+        const double us = split_time(items, units, s, slots, unit_sm, sms, rows * q_heads);
+        if (us < least) {
+            least = us;
+            best = s;
+        }
+    };
+    for (int64_t s = 1; s <= units && (s - 1) * items <= 3 * slots; s += 1 + s / 8) consider(s);
+    for (int64_t w = 1; w <= 3; ++w)  // parts that fill whole waves
+        if (const int64_t s = w * slots / items; s > 1 && s <= units) consider(s);
+    if (items * best > INT32_MAX) return fail(TIR_ERR_UNSUPPORTED_SHAPE, "tir_paged_attention: too many rows");
+    p->splits = static_cast<int32_t>(best);
+    p->min_units = 1;
     return TIR_OK;
 }
 

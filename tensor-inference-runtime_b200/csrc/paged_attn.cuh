@@ -81,6 +81,10 @@ __device__ __forceinline__ int32_t row_length(const AttnArgs& a, const PagesView
 }
 
 // ---- instruction wrappers ----------------------------------------------------
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // Copies 16 bytes, or (size 0) writes zeros and reads nothing.
 __device__ __forceinline__ void cp_async16_sized(uint32_t dst, const void* src, int size) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
@@ -108,7 +112,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t* r, uint32_t addr) {
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 
@@ -116,12 +120,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 template <bool BF>
 __device__ __forceinline__ void mma16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     if constexpr (BF)
-        asm volatile(
+        asm(
             "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile(
+        asm(
             "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -129,7 +133,7 @@ __device__ __forceinline__ void mma16(float* d, const uint32_t* a, uint32_t b0, 
 
 // d (16 x 8, f32) += a (16 x 8) b (8 x 8), tf32 operands
 __device__ __forceinline__ void mma8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -161,6 +165,15 @@ __device__ __forceinline__ void q8_pairs(uint32_t w, uint32_t* even, uint32_t* o
     const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
     *even = *reinterpret_cast<const uint32_t*>(&x);
     *odd = *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// The same as (128 + n) 2^-24, f16's denormals: three operations instead of five
+// where the 128 can be taken off the sum (the keys: by what an accumulator starts
+// from; it is of the sum's own size there, so nothing is lost to it.  The values'
+// sums run over the positions, where it would outgrow them).
+__device__ __forceinline__ void q8_pairs_biased(uint32_t w, uint32_t* even, uint32_t* odd) {
+    *even = (w & 0x00ff00ffu) ^ 0x00800080u;
+    *odd = ((w >> 8) & 0x00ff00ffu) ^ 0x00800080u;
 }
 
 // The Q8_0 steps of one position's head: D / 32 halves in one load.
@@ -211,29 +224,29 @@ struct AttnCfg {
     static constexpr int MT = TILE / 16;
     static constexpr int PITCH = ROW + 16;  // an odd number of 16-byte units: ldmatrix rows fall on different banks
     static constexpr int STEPS = q8 ? D / 32 * 2 : 0;  // bytes of a position's Q8_0 steps
-    static constexpr int V_AT = TILE * PITCH;
-    static constexpr int KS_AT = 2 * TILE * PITCH, VS_AT = KS_AT + TILE * STEPS;
-    static constexpr int STAGE = KS_AT + 2 * TILE * STEPS;
+    static constexpr int STEPS_AT = TILE * PITCH;
+    static constexpr int HALF = STEPS_AT + TILE * STEPS;  // the keys or the values of a tile
     static constexpr int KSTEPS = tf32 ? D / 8 : D / 16;  // q operand steps
     static constexpr int QBYTES = KSTEPS * NT * NQ * 256;
     static constexpr int HEADS = 8 * NT;
-    static constexpr int WARPS = STAGE > 32 * 1024 ? 2 : 4;
+    static constexpr int WARPS = HALF > 16 * 1024 && NT == 2 ? 2 : 4;  // two where q takes the room
     static constexpr int THREADS = WARPS * 32;
     static constexpr int UNIT = WARPS * TILE;
-    static constexpr int FIXED = QBYTES + HEADS * 4 + WARPS * HEADS * 8;
-    // two CTAs an SM where three stages fit in half of its shared memory, else one
-    static constexpr int half_stages = (112 * 1024 - FIXED) / (WARPS * STAGE);
-    static constexpr int full_stages = (224 * 1024 - FIXED) / (WARPS * STAGE);
-    static constexpr int PER_SM = half_stages >= 3 ? 2 : 1;
-    static constexpr int fit = PER_SM == 2 ? half_stages : full_stages;
-    static constexpr int STAGES = fit > 6 ? 6 : fit;
-    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int BIAS = q8 ? HEADS * (D / 32) * 4 : 0;
+    static constexpr int FIXED = QBYTES + HEADS * 4 + WARPS * HEADS * 8 + BIAS;
+    // a warp's ring: SLOTS half tiles (keys, values, keys, ...), an odd number, so that
+    // a step on keys asks for keys.  As many CTAs an SM as three slots each allow.
+    static constexpr int fits(int ctas) { return (227 * 1024 / ctas - 1024 - FIXED) / (WARPS * HALF); }
+    static constexpr int PER_SM = fits(3) >= 3 && D == 64 && NT == 1 ? 3 : fits(2) >= 3 ? 2 : 1;
+    static constexpr int SLOTS = fits(PER_SM) >= 7 ? 7 : fits(PER_SM) >= 5 ? 5 : 3;
+    static constexpr int AHEAD = (SLOTS - 1) / 2;  // tiles asked for before they are used
+    static constexpr int RING = WARPS * SLOTS * HALF;
     static constexpr int SMEM = RING + FIXED;
     // q operands in registers where they are few
     static constexpr bool q_in_regs = KSTEPS * NT * NQ * 2 <= 64;
-    static_assert(STAGES >= 2 && SMEM <= 227 * 1024, "the ring needs two stages");
-    static_assert(STAGES * STAGE >= HEADS * (D + 4) * 4, "a warp's output fits its ring");
-    static_assert(STAGE % 16 == 0 && RING % 16 == 0 && QBYTES % 16 == 0, "16-byte copies");
+    static_assert(fits(PER_SM) >= 3, "the ring needs three slots");
+    static_assert(SLOTS * HALF >= HEADS * (D + 4) * 4, "a warp's output fits its ring");
+    static_assert(HALF % 16 == 0 && RING % 16 == 0 && QBYTES % 16 == 0, "16-byte copies");
 };
 
 template <Elem C, int D, int NT, bool F32Q>
@@ -252,6 +265,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     uint32_t* qf = reinterpret_cast<uint32_t*>(smem + X::RING);
     float* cs = reinterpret_cast<float*>(smem + X::RING + X::QBYTES);
     float* ml = cs + X::HEADS;  // [WARPS][HEADS][2]
+    float* bias = ml + X::WARPS * X::HEADS * 2;  // Q8_0: [D / 32][HEADS]
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int tiles = kv.kv_heads * a.head_tiles;
@@ -281,7 +295,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     // ---- the ring ----
     const int n_tiles = (range.k1 - range.k0 + X::TILE - 1) / X::TILE;
     const int my_tiles = n_tiles > warp ? (n_tiles - warp + X::WARPS - 1) / X::WARPS : 0;
-    uint8_t* my_ring = ring + warp * X::STAGES * X::STAGE;
+    uint8_t* my_ring = ring + warp * X::SLOTS * X::HALF;
     const uint32_t ring_addr = smem_u32(my_ring);
     // this lane's position (lane % TILE) of the warp's tile i, and the page it is on:
     // asked for one tile before its copies are issued, checked only then
@@ -290,41 +304,56 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         const int32_t pos = position(i);
         return pos < range.k1 ? page_id(kv, row, pos) : -1;
     };
-    const int64_t head_at = static_cast<int64_t>(hk) * kv.head_stride;
-    const int64_t k_to_v = kv.v - kv.k;
-    auto issue = [&](int i, int slot, int32_t page) {
-        if (i < my_tiles) {
-            const int32_t pos = position(i);
-            int64_t mine = -1;
-            if (pos < range.k1 && page_ok(kv, page)) mine = slot_of(kv, page, pos) + head_at;
-            const uint32_t dst = ring_addr + slot * X::STAGE;
-            if constexpr (X::q8) {
-                const bool live = mine >= 0;
-                const int64_t at = live ? mine >> 5 : 0;
-                const uint32_t to = dst + (lane & (X::TILE - 1)) * X::STEPS;
-                if (X::TILE == 32 || lane < 16) cp_async_small_or_zero<X::STEPS>(to + X::KS_AT, kv.ks + at, live);
-                if (X::TILE == 32 || lane >= 16) cp_async_small_or_zero<X::STEPS>(to + X::VS_AT, kv.vs + at, live);
-            }
-            // a 128-byte line (or a whole shorter row) at a time
+    // where this lane's position of tile i lies, in 16-byte units; kNowhere past the
+    // end or on a bad page: zeros instead
+    constexpr uint32_t kNowhere = 0xffffffffu;
+    const uint32_t head_at = hk * kv.head16;
+    auto place = [&](int i, int32_t page) -> uint32_t {
+        const int32_t pos = position(i);
+        return pos < range.k1 && page_ok(kv, page) ? slot16_of(kv, page, pos) + head_at : kNowhere;
+    };
+    // copies the keys or values of a tile into a slot, a 128-byte line (or a whole
+    // shorter row) at a time
+    auto issue = [&](int slot, uint32_t mine, bool full, const char* pool, const uint16_t* steps) {
+        const uint32_t dst = ring_addr + slot * X::HALF;
+        if constexpr (X::q8) {
+            if (X::TILE == 32 || lane < 16)
+                cp_async_small_or_zero<X::STEPS>(dst + X::STEPS_AT + lane * X::STEPS, steps + (mine == kNowhere ? 0 : mine >> 1), mine != kNowhere);
+        }
+        const char* from = pool + (lane % LPR) * 16;
+        const uint32_t to = dst + (lane / LPR) * X::PITCH + (lane % LPR) * 16;
+        if (full) {
 #pragma unroll
             for (int u = 0; u < X::TILE * LPR / 32; ++u) {
-                const int key = u * (32 / LPR) + lane / LPR;
-                const int64_t at = __shfl_sync(FULL, mine, key);
-                const int size = at >= 0 ? 16 : 0;
-                const char* from = kv.k + (at >= 0 ? at * X::ES : 0) + (lane % LPR) * 16;
-                const uint32_t to = dst + key * X::PITCH + (lane % LPR) * 16;
+                const uint32_t at = __shfl_sync(FULL, mine, u * (32 / LPR) + lane / LPR);
+                const char* row_from = from + static_cast<uint64_t>(at) * 16;
 #pragma unroll
-                for (int ch = 0; ch < CH; ch += LPR) {
-                    cp_async16_sized(to + ch * 16, from + ch * 16, size);
-                    cp_async16_sized(to + X::V_AT + ch * 16, from + k_to_v + ch * 16, size);
-                }
+                for (int ch = 0; ch < CH; ch += LPR) cp_async16(to + u * (32 / LPR) * X::PITCH + ch * 16, row_from + ch * 16);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < X::TILE * LPR / 32; ++u) {
+                const uint32_t at = __shfl_sync(FULL, mine, u * (32 / LPR) + lane / LPR);
+                const char* row_from = from + (at == kNowhere ? 0 : static_cast<uint64_t>(at) * 16);
+#pragma unroll
+                for (int ch = 0; ch < CH; ch += LPR)
+                    cp_async16_sized(to + u * (32 / LPR) * X::PITCH + ch * 16, row_from + ch * 16, at == kNowhere ? 0 : 16);
             }
         }
-        cp_async_commit();
     };
+    int32_t pages[X::AHEAD + 1];  // all asked for before the first is waited for
 #pragma unroll
-    for (int i = 0; i < X::STAGES - 1; ++i) issue(i, i, lookup(i));
-    int32_t next_page = lookup(X::STAGES - 1);
+    for (int i = 0; i <= X::AHEAD; ++i) pages[i] = lookup(i);
+#pragma unroll
+    for (int i = 0; i < X::AHEAD; ++i) {
+        const uint32_t at = place(i, pages[i]);
+        const bool full = __all_sync(FULL, at != kNowhere);
+        if (i < my_tiles) issue(2 * i, at, full, kv.k, kv.ks);
+        cp_async_commit();
+        if (i < my_tiles) issue(2 * i + 1, at, full, kv.v, kv.vs);
+        cp_async_commit();
+    }
+    int32_t next_page = pages[X::AHEAD];
 
     // ---- q operands, while the first tiles are on their way ----
     for (int j = warp; j < X::HEADS; j += X::WARPS) {
@@ -355,6 +384,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                 for (int i = 0; i < D / 32; ++i) x[i] *= up;
             }
         }
+        if constexpr (X::q8) c *= 16777216.f;  // the keys' 2^-24
         if (lane == 0) cs[j] = fmaxf(c, 1.2e-38f);  // never 0: a masked score is c * -inf
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -381,6 +411,12 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                         *p = __half_as_ushort(b);
                         rem -= __half2float(b);
                     }
+                }
+                if constexpr (X::q8) {
+                    float sum = x[i] - rem;  // what the parts hold
+#pragma unroll
+                    for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(FULL, sum, w);
+                    if (lane == 0) bias[i * X::HEADS + j] = -128.f / 16777216.f * sum;
                 }
             }
         }
@@ -416,6 +452,15 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+    float off[X::q8 ? D / 32 : 1][NT][2];
+    if constexpr (X::q8) {
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) off[b][n][e] = bias[b * X::HEADS + n * 8 + 2 * t + e];
+    }
     int v_exp = 0;  // Q8_0: o is kept over 2^(v_exp - 14), the power of two above the steps seen so far
 
     // c s - base.  The product is rounded (or exact: c is a power of two under f32
@@ -428,54 +473,66 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     };
 
     // ---- the loop over this warp's tiles ----
-    int slot = 0, free_slot = X::STAGES - 1;
-    for (int it = 0; it < my_tiles; ++it) {
-        cp_async_wait<X::STAGES - 2>();
-        __syncwarp();
-        issue(it + X::STAGES - 1, free_slot, next_page);
-        next_page = lookup(it + X::STAGES);
-        const uint8_t* st = my_ring + slot * X::STAGE;
-        const uint32_t sa = ring_addr + slot * X::STAGE;
+    int slot = 0, free_slot = X::SLOTS - 1;
+    auto advance = [&]() {
         free_slot = slot;
-        slot = slot + 1 == X::STAGES ? 0 : slot + 1;
-        const uint32_t row_addr = sa + (lane & 15) * X::PITCH + (lane >> 4) * 16;
+        slot = slot + 1 == X::SLOTS ? 0 : slot + 1;
+    };
+    for (int it = 0; it < my_tiles; ++it) {
+        cp_async_wait<X::SLOTS - 2>();
+        __syncwarp();
+        const bool more = it + X::AHEAD < my_tiles;
+        const uint32_t ahead = place(it + X::AHEAD, next_page);
+        const bool full = __all_sync(FULL, ahead != kNowhere);
+        if (more) issue(free_slot, ahead, full, kv.k, kv.ks);
+        cp_async_commit();
+        next_page = lookup(it + X::AHEAD + 1);
+        const uint8_t* st = my_ring + slot * X::HALF;
+        const uint32_t row_addr = ring_addr + slot * X::HALF + (lane & 15) * X::PITCH + (lane >> 4) * 16;
+        advance();
 
         // S' = K Q'
         float s[X::MT][NT][4];
 #pragma unroll
         for (int mt = 0; mt < X::MT; ++mt) {
             const uint32_t k_addr = row_addr + mt * 16 * X::PITCH;
-            float s2[NT][4];
+            // several sums at once: a product waits for the one before it in its chain
+            constexpr int CHAINS = X::q8 ? 1 : X::tf32 ? 6 : 2 * X::NQ;
+            float acc[CHAINS][NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[mt][n][e] = s2[n][e] = 0.f;
+                for (int e = 0; e < 4; ++e) {
+                    s[mt][n][e] = 0.f;
+#pragma unroll
+                    for (int x = 0; x < CHAINS; ++x) acc[x][n][e] = 0.f;
+                }
             if constexpr (X::q8) {
                 Steps<D> k_steps[2];
-                k_steps[0].load(st + X::KS_AT, mt * 16 + g);
-                k_steps[1].load(st + X::KS_AT, mt * 16 + g + 8);
+                k_steps[0].load(st + X::STEPS_AT, mt * 16 + g);
+                k_steps[1].load(st + X::STEPS_AT, mt * 16 + g + 8);
 #pragma unroll
                 for (int b = 0; b < D / 32; ++b) {
                     uint32_t w[4], x0[4], x1[4];
                     ldsm4(w, k_addr + b * 32);
-                    q8_pairs(w[0], &x0[0], &x0[2]);
-                    q8_pairs(w[1], &x0[1], &x0[3]);
-                    q8_pairs(w[2], &x1[0], &x1[2]);
-                    q8_pairs(w[3], &x1[1], &x1[3]);
+                    q8_pairs_biased(w[0], &x0[0], &x0[2]);
+                    q8_pairs_biased(w[1], &x0[1], &x0[3]);
+                    q8_pairs_biased(w[2], &x1[0], &x1[2]);
+                    q8_pairs_biased(w[3], &x1[1], &x1[3]);
                     const float d0 = k_steps[0].get(b), d1 = k_steps[1].get(b);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                        float sum[4] = {off[b][n][0], off[b][n][1], off[b][n][0], off[b][n][1]};
 #pragma unroll
                         for (int p = X::NQ - 1; p >= 0; --p) {
                             const uint2 q0 = q_op(2 * b, n, p), q1 = q_op(2 * b + 1, n, p);
-                            mma16<false>(acc, x0, q0.x, q0.y);
-                            mma16<false>(acc, x1, q1.x, q1.y);
+                            mma16<false>(sum, x0, q0.x, q0.y);
+                            mma16<false>(sum, x1, q1.x, q1.y);
                         }
-                        s[mt][n][0] = fmaf(acc[0], d0, s[mt][n][0]);
-                        s[mt][n][1] = fmaf(acc[1], d0, s[mt][n][1]);
-                        s[mt][n][2] = fmaf(acc[2], d1, s[mt][n][2]);
-                        s[mt][n][3] = fmaf(acc[3], d1, s[mt][n][3]);
+                        s[mt][n][0] = fmaf(sum[0], d0, s[mt][n][0]);
+                        s[mt][n][1] = fmaf(sum[1], d0, s[mt][n][1]);
+                        s[mt][n][2] = fmaf(sum[2], d1, s[mt][n][2]);
+                        s[mt][n][3] = fmaf(sum[3], d1, s[mt][n][3]);
                     }
                 }
             } else if constexpr (X::tf32) {
@@ -488,9 +545,9 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         const uint2 qh = q_op(kk, n, 0), ql = q_op(kk, n, 1);
-                        mma8(s2[n], lo, qh.x, qh.y);
-                        mma8(s2[n], hi, ql.x, ql.y);
-                        mma8(s[mt][n], hi, qh.x, qh.y);
+                        mma8(acc[kk & 1][n], lo, qh.x, qh.y);
+                        mma8(acc[2 + (kk & 1)][n], hi, ql.x, ql.y);
+                        mma8(acc[4 + (kk & 1)][n], hi, qh.x, qh.y);
                     }
                 }
             } else {
@@ -503,7 +560,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 #pragma unroll
                         for (int p = X::NQ - 1; p >= 0; --p) {
                             const uint2 qv = q_op(kk, n, p);
-                            mma16<X::bf>(((kk + p) & 1) ? s2[n] : s[mt][n], w, qv.x, qv.y);
+                            mma16<X::bf>(acc[2 * (X::NQ - 1 - p) + (kk & 1)][n], w, qv.x, qv.y);
                         }
                 }
             }
@@ -511,7 +568,11 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[mt][n][e] += s2[n][e];
+                    for (int e = 0; e < 4; ++e) {
+                        // smallest parts first
+#pragma unroll
+                        for (int x = 0; x < CHAINS; ++x) s[mt][n][e] += acc[x][n][e];
+                    }
             }
         }
 
@@ -539,6 +600,14 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                 if constexpr (!X::plain) top[n][e] *= c[n][e];
                 moves |= top[n][e] > m[n][e] + kLag;
             }
+        // the values' turn
+        cp_async_wait<X::SLOTS - 2>();
+        __syncwarp();
+        if (more) issue(free_slot, ahead, full, kv.v, kv.vs);
+        cp_async_commit();
+        const uint8_t* sv = my_ring + slot * X::HALF;
+        const uint32_t v_base = ring_addr + slot * X::HALF;
+        advance();
         Steps<X::q8 ? D : 64> v_steps[X::MT][2];
         uint32_t v_top = 0u;
         if constexpr (X::q8) {
@@ -546,7 +615,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
             for (int mt = 0; mt < X::MT; ++mt)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    v_steps[mt][half].load(st + X::VS_AT, mt * 16 + g + 8 * half);
+                    v_steps[mt][half].load(sv + X::STEPS_AT, mt * 16 + g + 8 * half);
                     v_top = __vmaxu2(v_top, v_steps[mt][half].top());
                 }
             v_top = max(v_top & 0xffffu, v_top >> 16) >> 10;
@@ -599,7 +668,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         for (int mt = 0; mt < X::MT; ++mt) {
             if constexpr (X::q8) {
                 const float inv = __uint_as_float(static_cast<uint32_t>(127 + 14 - v_exp) << 23);
-                const uint32_t v_addr = row_addr + X::V_AT + mt * 16 * X::PITCH;
+                const uint32_t v_addr = v_base + (mt * 16 + (lane & 15)) * X::PITCH + (lane >> 4) * 16;
 #pragma unroll
                 for (int b = 0; b < D / 32; ++b) {
                     const float d0 = v_steps[mt][0].get(b) * inv, d1 = v_steps[mt][1].get(b) * inv;
@@ -614,19 +683,21 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                         p1[n][0] = transpose8x8(pack2(w0 - fa.x, w1 - fa.y, Elem::F16));
                         p1[n][1] = transpose8x8(pack2(w2 - fb.x, w3 - fb.y, Elem::F16));
                     }
-                    uint32_t w[4];
+                    uint32_t w[4], x[2][4];
                     ldsm4_t(w, v_addr + b * 32);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        uint32_t x[4];
-                        q8_pairs(w[2 * i], &x[0], &x[1]);
-                        q8_pairs(w[2 * i + 1], &x[2], &x[3]);
+                        q8_pairs(w[2 * i], &x[i][0], &x[i][1]);
+                        q8_pairs(w[2 * i + 1], &x[i][2], &x[i][3]);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma16<false>(o[2 * b + i][n], x, p1[n][0], p1[n][1]);
-                            mma16<false>(o[2 * b + i][n], x, p0[n][0], p0[n][1]);
+                            mma16<false>(o[2 * b + i][n], x[i], p1[n][0], p1[n][1]);
                         }
                     }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma16<false>(o[2 * b + i][n], x[i], p0[n][0], p0[n][1]);
                 }
             } else if constexpr (X::tf32) {
 #pragma unroll
@@ -639,7 +710,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                         split_tf32(__uint_as_float(__byte_perm(dn, up, 0x5410)), &ph[n][0], &pl[n][0]);
                         split_tf32(__uint_as_float(__byte_perm(dn, up, 0x7632)), &ph[n][1], &pl[n][1]);
                     }
-                    const uint8_t* v = st + X::V_AT + (mt * 16 + 8 * kb + 2 * t) * X::PITCH + g * 8;
+                    const uint8_t* v = sv + (mt * 16 + 8 * kb + 2 * t) * X::PITCH + g * 8;
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) {
                         const float2 va = *reinterpret_cast<const float2*>(v + i * 64);
@@ -671,7 +742,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                         r0 -= fa.x, r1 -= fa.y, r2 -= fb.x, r3 -= fb.y;
                     }
                 }
-                const uint32_t v_addr = sa + X::V_AT + (mt * 16 + (lane & 7) + (lane >> 4) * 8) * X::PITCH + ((lane >> 3) & 1) * 16;
+                const uint32_t v_addr = v_base + (mt * 16 + (lane & 7) + (lane >> 4) * 8) * X::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
                     uint32_t w[4];
@@ -733,7 +804,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
             const float f = mw == -INFINITY ? 0.f : exp2_fast(mw - top);
             const float lw = ml[(w * X::HEADS + j) * 2 + 1];
             sum += f * lw;
-            const float* part = reinterpret_cast<const float*>(ring + w * X::STAGES * X::STAGE) + j * (D + 4) + d;
+            const float* part = reinterpret_cast<const float*>(ring + w * X::SLOTS * X::HALF) + j * (D + 4) + d;
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = fmaf(f, part[e], y[e]);
         }
@@ -766,15 +837,17 @@ cudaError_t launch_attn_as(const AttnArgs& a, const PagesView& kv, int64_t rows,
 }
 
 // Geometry of the kernel that a cache type, head size and query type get: CTAs
-// an SM holds, and the positions of a unit.
+// an SM holds, the positions of a unit, and what an element weighs in bytes.
 struct AttnShape {
     int per_sm, unit;
+    double bytes;
 };
 
 template <Elem C, int D, bool F32Q>
 AttnShape attn_shape_as(int nt) {
-    if (nt == 1) return {AttnCfg<C, D, 1, F32Q>::PER_SM, AttnCfg<C, D, 1, F32Q>::UNIT};
-    return {AttnCfg<C, D, 2, F32Q>::PER_SM, AttnCfg<C, D, 2, F32Q>::UNIT};
+    const double bytes = C == Elem::Q8 ? 1.5 * 34 / 32 : ElemOf<C>::bytes;
+    if (nt == 1) return {AttnCfg<C, D, 1, F32Q>::PER_SM, AttnCfg<C, D, 1, F32Q>::UNIT, bytes};
+    return {AttnCfg<C, D, 2, F32Q>::PER_SM, AttnCfg<C, D, 2, F32Q>::UNIT, bytes};
 }
 
 // One function per cache type (paged_attn_<type>.cu): the launch, or with `shape`

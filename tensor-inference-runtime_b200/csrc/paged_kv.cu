@@ -337,6 +337,13 @@ tir_status pages_view(const tir_kv_pages* kv, const char* entry, PagesView* v, E
     if ((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v) |
          (q8 ? reinterpret_cast<uintptr_t>(kv->k_scale) | reinterpret_cast<uintptr_t>(kv->v_scale) : 0)) % 16)
         return fail(TIR_ERR_INVALID_ARG, who + ": pools must be 16-byte aligned");
+    const int es = elem_bytes(*type);
+    const double span = (static_cast<double>(kv->n_pages) * kv->page_stride + static_cast<double>(kv->page_size) * kv->pos_stride +
+                         static_cast<double>(kv->kv_heads) * kv->head_stride) * es / 16;
+    if (span >= 4294967295.0) return fail(TIR_ERR_UNSUPPORTED_SHAPE, who + ": a pool spans 64 GB or more");
+    v->page16 = static_cast<uint32_t>(kv->page_stride * es / 16);
+    v->pos16 = static_cast<uint32_t>(kv->pos_stride * es / 16);
+    v->head16 = static_cast<uint32_t>(kv->head_stride * es / 16);
     v->k = static_cast<char*>(kv->k);
     v->v = static_cast<char*>(kv->v);
     v->ks = kv->k_scale;
