@@ -663,14 +663,29 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                     l[n][e] += s[mt][n][e] + s[mt][n][e + 2];
                 }
 
-        // O' += V' P'
+        // O' += V' P'.  The tensor core's f32 sums are cut off, not rounded: under f32
+        // queries a tile's products are summed from zero and then added, so that a
+        // long row's error does not grow with its length.
+        auto begin = [&](float* acc, const float* sum) {
 #pragma unroll
-        for (int mt = 0; mt < X::MT; ++mt) {
-            if constexpr (X::q8) {
-                const float inv = __uint_as_float(static_cast<uint32_t>(127 + 14 - v_exp) << 23);
-                const uint32_t v_addr = v_base + (mt * 16 + (lane & 15)) * X::PITCH + (lane >> 4) * 16;
+            for (int e = 0; e < 4; ++e) acc[e] = F32Q ? 0.f : sum[e];
+        };
+        auto finish = [&](float* sum, const float* acc) {
 #pragma unroll
-                for (int b = 0; b < D / 32; ++b) {
+            for (int e = 0; e < 4; ++e) sum[e] = F32Q ? sum[e] + acc[e] : acc[e];
+        };
+        if constexpr (X::q8) {
+            const float inv = __uint_as_float(static_cast<uint32_t>(127 + 14 - v_exp) << 23);
+            const uint32_t v_addr = v_base + (lane & 15) * X::PITCH + (lane >> 4) * 16;
+#pragma unroll
+            for (int b = 0; b < D / 32; ++b) {
+                float acc[2][NT][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) begin(acc[i][n], o[2 * b + i][n]);
+#pragma unroll
+                for (int mt = 0; mt < X::MT; ++mt) {
                     const float d0 = v_steps[mt][0].get(b) * inv, d1 = v_steps[mt][1].get(b) * inv;
                     uint32_t p0[NT][2], p1[NT][2];
 #pragma unroll
@@ -684,37 +699,49 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                         p1[n][1] = transpose8x8(pack2(w2 - fb.x, w3 - fb.y, Elem::F16));
                     }
                     uint32_t w[4], x[2][4];
-                    ldsm4_t(w, v_addr + b * 32);
+                    ldsm4_t(w, v_addr + mt * 16 * X::PITCH + b * 32);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         q8_pairs(w[2 * i], &x[i][0], &x[i][1]);
                         q8_pairs(w[2 * i + 1], &x[i][2], &x[i][3]);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            mma16<false>(o[2 * b + i][n], x[i], p1[n][0], p1[n][1]);
-                        }
+                        for (int n = 0; n < NT; ++n) mma16<false>(acc[i][n], x[i], p1[n][0], p1[n][1]);
                     }
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma16<false>(o[2 * b + i][n], x[i], p0[n][0], p0[n][1]);
+                        for (int n = 0; n < NT; ++n) mma16<false>(acc[i][n], x[i], p0[n][0], p0[n][1]);
                 }
-            } else if constexpr (X::tf32) {
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    uint32_t ph[NT][2], pl[NT][2];
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) finish(o[2 * b + i][n], acc[i][n]);
+            }
+        } else if constexpr (X::tf32) {
+            uint32_t ph[X::MT][2][NT][2], pl[X::MT][2][NT][2];
+#pragma unroll
+            for (int mt = 0; mt < X::MT; ++mt)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         const uint32_t x = __float_as_uint(s[mt][n][2 * kb]), y = __float_as_uint(s[mt][n][2 * kb + 1]);
                         const uint32_t up = transpose8x8(__byte_perm(x, y, 0x7632)), dn = transpose8x8(__byte_perm(x, y, 0x5410));
-                        split_tf32(__uint_as_float(__byte_perm(dn, up, 0x5410)), &ph[n][0], &pl[n][0]);
-                        split_tf32(__uint_as_float(__byte_perm(dn, up, 0x7632)), &ph[n][1], &pl[n][1]);
+                        split_tf32(__uint_as_float(__byte_perm(dn, up, 0x5410)), &ph[mt][kb][n][0], &pl[mt][kb][n][0]);
+                        split_tf32(__uint_as_float(__byte_perm(dn, up, 0x7632)), &ph[mt][kb][n][1], &pl[mt][kb][n][1]);
                     }
-                    const uint8_t* v = sv + (mt * 16 + 8 * kb + 2 * t) * X::PITCH + g * 8;
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        const float2 va = *reinterpret_cast<const float2*>(v + i * 64);
-                        const float2 vb = *reinterpret_cast<const float2*>(v + X::PITCH + i * 64);
+            for (int i = 0; i < D / 16; ++i) {
+                float acc[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) begin(acc[n], o[i][n]);
+#pragma unroll
+                for (int mt = 0; mt < X::MT; ++mt)
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) {
+                        const uint8_t* v = sv + (mt * 16 + 8 * kb + 2 * t) * X::PITCH + g * 8 + i * 64;
+                        const float2 va = *reinterpret_cast<const float2*>(v);
+                        const float2 vb = *reinterpret_cast<const float2*>(v + X::PITCH);
                         uint32_t hi[4], lo[4];
                         split_tf32(va.x, &hi[0], &lo[0]);
                         split_tf32(va.y, &hi[1], &lo[1]);
@@ -722,36 +749,47 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                         split_tf32(vb.y, &hi[3], &lo[3]);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma8(o[i][n], lo, ph[n][0], ph[n][1]);
-                            mma8(o[i][n], hi, pl[n][0], pl[n][1]);
-                            mma8(o[i][n], hi, ph[n][0], ph[n][1]);
+                            mma8(acc[n], lo, ph[mt][kb][n][0], ph[mt][kb][n][1]);
+                            mma8(acc[n], hi, pl[mt][kb][n][0], pl[mt][kb][n][1]);
+                            mma8(acc[n], hi, ph[mt][kb][n][0], ph[mt][kb][n][1]);
                         }
                     }
-                }
-            } else {
-                uint32_t pp[NT][X::NP][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) finish(o[i][n], acc[n]);
+            }
+        } else {
+            uint32_t pp[X::MT][NT][X::NP][2];
+#pragma unroll
+            for (int mt = 0; mt < X::MT; ++mt)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float r0 = s[mt][n][0], r1 = s[mt][n][1], r2 = s[mt][n][2], r3 = s[mt][n][3];
 #pragma unroll
                     for (int p = 0; p < X::NP; ++p) {
                         const uint32_t wa = pack2(r0, r1, C), wb = pack2(r2, r3, C);
-                        pp[n][p][0] = transpose8x8(wa);
-                        pp[n][p][1] = transpose8x8(wb);
+                        pp[mt][n][p][0] = transpose8x8(wa);
+                        pp[mt][n][p][1] = transpose8x8(wb);
                         const float2 fa = unpack2(wa, C), fb = unpack2(wb, C);
                         r0 -= fa.x, r1 -= fa.y, r2 -= fb.x, r3 -= fb.y;
                     }
                 }
-                const uint32_t v_addr = v_base + (mt * 16 + (lane & 7) + (lane >> 4) * 8) * X::PITCH + ((lane >> 3) & 1) * 16;
+            const uint32_t v_addr = v_base + ((lane & 7) + (lane >> 4) * 8) * X::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
+            for (int i = 0; i < D / 16; ++i) {
+                float acc[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) begin(acc[n], o[i][n]);
+#pragma unroll
+                for (int mt = 0; mt < X::MT; ++mt) {
                     uint32_t w[4];
-                    ldsm4_t(w, v_addr + i * 32);
+                    ldsm4_t(w, v_addr + mt * 16 * X::PITCH + i * 32);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int p = X::NP - 1; p >= 0; --p) mma16<X::bf>(o[i][n], w, pp[n][p][0], pp[n][p][1]);
+                        for (int p = X::NP - 1; p >= 0; --p) mma16<X::bf>(acc[n], w, pp[mt][n][p][0], pp[mt][n][p][1]);
                 }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) finish(o[i][n], acc[n]);
             }
         }
     }
