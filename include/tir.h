@@ -447,7 +447,7 @@ enum { TIR_PAIRS_ADJACENT = 0, TIR_PAIRS_HALVES = 1 };
  * 141-150 with this eps and weight; NULL weight: none), then the rotation of
  * its first rope_dim elements (a multiple of 16; rope NULL: none) by the cos
  * and sin in row `position` of a device table [rope_positions][rope_dim / 2][2]
- * (tir_rope_table). */
+ * (tir_rope_table).  Weights and table are 16-byte aligned. */
 typedef struct tir_qk_norm {
     const float *q_weight, *k_weight;
     const float *rope;

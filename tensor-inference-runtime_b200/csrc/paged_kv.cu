@@ -39,7 +39,10 @@ struct RowArgs {
     const int32_t *seqs, *positions;
     int64_t tokens;
     int32_t q_heads, kv_heads;
-    int32_t heads;  // of a token: q_heads + kv_heads (+ kv_heads values, when appending)
+    int32_t kinds;  // of key-value heads: keys, or keys and values
+    // chunks of a token's heads, none of two kinds: all of them, of queries, of keys
+    uint32_t chunks;
+    int32_t q_chunks, kv_chunks;
     const float *q_w, *k_w, *rope;
     int64_t rope_positions;
     int32_t rope_dim, pairs;
@@ -47,186 +50,272 @@ struct RowArgs {
     uint32_t* err;
 };
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {  // within one ulp
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // One Q8_0 block's rule (activated_q8, src/kernels.rs:8-31) over the four lanes
 // that hold its 32 values: step = the last of the elements of largest |x| / 127,
 // quants = round half away (x / step), saturated, NaN -> 0.  The quotient uses
-// the step before it is rounded to f16, as there.  IEEE divisions keep the
-// quants equal to tir_activated_q8's.
+// the step before it is rounded to f16, as there, and the quants equal
+// tir_activated_q8's bit for bit:
+// * the largest and the smallest value give the step's sign, unless both reach
+//   the largest magnitude; then the elements' order decides (a zero block, too);
+// * x * (1 / step) is within 127 * 2^-22 < 2^-14 of the quotient, so where it is
+//   further than that from a half its nearest integer is the quotient's; nearer,
+//   and for steps too small or too large to invert, x is divided.
 __device__ __forceinline__ void quantise8(const float* f, int lane4, uint2* quants, float* step) {
-    uint32_t top = 0u;
+    float hi = f[0], lo = -f[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(FULL, top, 1));
-    top = max(top, __shfl_xor_sync(FULL, top, 2));
-    uint32_t last = 0u;  // 2 (index + 1) + sign of the last element of magnitude `top`
+    for (int i = 1; i < 8; ++i) {
+        hi = max_nan(hi, f[i]);
+        lo = max_nan(lo, -f[i]);
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if ((__float_as_uint(f[i]) & 0x7fffffffu) == top) last = 2u * (lane4 * 8 + i + 1) + (__float_as_uint(f[i]) >> 31);
-    last = max(last, __shfl_xor_sync(FULL, last, 1));
-    last = max(last, __shfl_xor_sync(FULL, last, 2));
-    const float d = __fdiv_rn(__uint_as_float(top | (last << 31)), 127.0f);
+    for (int w = 1; w <= 2; w <<= 1) {
+        hi = max_nan(hi, __shfl_xor_sync(FULL, hi, w));
+        lo = max_nan(lo, __shfl_xor_sync(FULL, lo, w));
+    }
+    float top = hi > lo ? hi : -lo;  // NaN: -lo, NaN as well
+    if (__any_sync(FULL, hi == lo)) {
+        uint32_t last = 0u;  // 2 (index + 1) + sign of the last element of magnitude hi
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (fabsf(f[i]) == hi) last = 2u * (lane4 * 8 + i + 1) + (__float_as_uint(f[i]) >> 31);
+        last = max(last, __shfl_xor_sync(FULL, last, 1));
+        last = max(last, __shfl_xor_sync(FULL, last, 2));
+        if (hi == lo) top = last & 1u ? -hi : hi;
+    }
+    const float d = __fdiv_rn(top, 127.0f);
+    const float inv = rcp_approx(d);
+    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: a sum with it has the nearest integer in its low bits
+    float far = 0.f;
     uint32_t b[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float r = roundf(__fdiv_rn(f[i], d));
-        const int n = r != r ? 0 : static_cast<int>(fminf(fmaxf(r, -128.f), 127.f));
-        b[i] = static_cast<uint32_t>(n) & 0xffu;
+        const float r = __fmul_rn(f[i], inv), n = __fadd_rn(r, kRound);
+        b[i] = __float_as_uint(n);
+        far = fmaxf(far, fabsf(r - (n - kRound)));
     }
-    quants->x = b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24);
-    quants->y = b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24);
+    if (!(far < 0.5f - 1.0f / 16384.0f && fabsf(d) >= 1e-36f && fabsf(d) <= 1e36f)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float r = roundf(__fdiv_rn(f[i], d));
+            b[i] = r != r ? 0u : static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(r, -128.f), 127.f)));
+        }
+    }
+    quants->x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    quants->y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
     *step = d;
 }
 
-// Writes this lane's eight elements of a head to element offset `at` of a pool.
-// Every lane of the warp calls it (the block maxima are shuffles).
-__device__ __forceinline__ void store_cache8(const float* f, bool live, Elem type, char* pool, uint16_t* scales,
-                                             int64_t at, int gl) {
-    if (type == Elem::Q8) {
-        uint2 w;
-        float step;
-        quantise8(f, gl & 3, &w, &step);
-        if (live) {
-            *reinterpret_cast<uint2*>(pool + at) = w;
-            if ((gl & 3) == 0) scales[at >> 5] = __half_as_ushort(__float2half_rn(step));
-        }
-    } else if (live) {
-        if (type == Elem::F32)
-            store8_as<Elem::F32>(pool + at * 4, f);
-        else if (type == Elem::F16)
-            store8_as<Elem::F16>(pool + at * 2, f);
-        else
-            store8_as<Elem::BF16>(pool + at * 2, f);
+// The cached slot of token t; false (and the error bit) outside the table or
+// on a bad page.
+__device__ __forceinline__ bool find_slot(const RowArgs& a, const PagesView& kv, int64_t row, int32_t pos, bool tell, int64_t* at) {
+    if (row < 0 || row >= kv.table_rows || pos >= static_cast<int64_t>(kv.max_pages) * kv.page_size) {
+        if (tell) atomicOr(a.err, kBadPosition);
+        return false;
     }
+    const int32_t id = page_of(kv, row, pos);
+    if (id < 0) return false;
+    *at = slot_of(kv, id, pos);
+    return true;
 }
 
-// Group of D / 8 lanes per (token, head).  kAppend: keys and values go to the
-// cache, else keys go to rows and there are no values.
-template <Elem A, int D, bool kAppend>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(const RowArgs a, const PagesView kv, const Elem cache) {
+// A group of D / 8 lanes takes HPG heads of one kind (queries, keys or values) of
+// a token.  With many tokens HPG = 4: their loads are in flight together, and the
+// token's position, slot, angles and weights are read once for four heads; with
+// few, HPG = 1 spreads them.  The heads' data are asked for before the slot is
+// looked up.  kAppend: keys and values go to the cache, else keys go to rows and
+// there are no values.
+template <Elem A, int D, bool kAppend, int HPG>
+__global__ void __launch_bounds__(kRowThreads, HPG == 4 ? 3 : 4) rows_kernel(const RowArgs a, const PagesView kv, const Elem cache) {
     constexpr int G = D / 8;
     constexpr int AB = ElemOf<A>::bytes;
     const int gl = threadIdx.x % G;
-    const int64_t item = (blockIdx.x * static_cast<int64_t>(kRowThreads) + threadIdx.x) / G;
-    const int64_t t = item / a.heads;
-    const int h = static_cast<int>(item % a.heads);
-    bool live = t < a.tokens;
-    const int32_t pos = live && a.positions ? a.positions[t] : 0;
-    if (pos < 0) live = false;
-    const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;
-    const int hk = is_q ? h : is_k ? h - a.q_heads : h - a.q_heads - a.kv_heads;
-    const bool turns = a.rope && (is_q || is_k);
+    const uint32_t item = (blockIdx.x * static_cast<uint32_t>(kRowThreads) + threadIdx.x) / G;
+    const uint32_t t = item / a.chunks;
+    int chunk = static_cast<int>(item % a.chunks);
+    const bool is_q = chunk < a.q_chunks;
+    if (!is_q) chunk -= a.q_chunks;
+    const bool is_v = !is_q && chunk >= a.kv_chunks;
+    if (is_v) chunk -= a.kv_chunks;
+    const int h0 = chunk * HPG, n = t < a.tokens ? min((is_q ? a.q_heads : a.kv_heads) - h0, HPG) : 0;
+    const int32_t pos = n > 0 && a.positions ? a.positions[t] : 0;
+    const int32_t seq = kAppend && n > 0 && a.seqs ? a.seqs[t] : static_cast<int32_t>(t);
+    const char* src = (is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + (h0 * D + gl * 8) * AB;
+    Raw8<A> raw[HPG];
+#pragma unroll
+    for (int x = 0; x < HPG; ++x) {
+        raw[x] = Raw8<A>{};
+        if (x < n) raw[x] = load_raw8<A>(src + x * D * AB);
+    }
+    const float* w_of = is_q ? a.q_w : is_v ? nullptr : a.k_w;
+    float4 w[2];
+    if (w_of) {
+        w[0] = reinterpret_cast<const float4*>(w_of)[gl * 2];
+        w[1] = reinterpret_cast<const float4*>(w_of)[gl * 2 + 1];
+    }
+    bool live = n > 0 && pos >= 0;
     if (live && a.rope && pos >= a.rope_positions) {
         if (gl == 0) atomicOr(a.err, kBadPosition);
         live = false;
     }
-    // where it goes
-    int64_t at = 0;
-    if (kAppend && live && !is_q) {
-        const int64_t row = a.seqs ? a.seqs[t] : t;
-        const int64_t cap = static_cast<int64_t>(kv.max_pages) * kv.page_size;
-        if (row < 0 || row >= kv.table_rows || pos >= cap) {
-            if (gl == 0) atomicOr(a.err, kBadPosition);
-            live = false;
-        } else {
-            const int32_t id = page_of(kv, row, pos);
-            live = id >= 0;
-            at = slot_of(kv, id, pos) + hk * kv.head_stride + gl * 8;
+    // angles of this lane's elements: four pairs, or with paired halves eight
+    const int half8 = a.rope_dim / 16;  // lanes of one half of the rotated elements
+    const bool halves = a.pairs == TIR_PAIRS_HALVES, turns = live && !is_v && gl < 2 * half8;
+    float4 cs[4];
+    if (turns) {
+        const float* p = a.rope + static_cast<int64_t>(pos) * a.rope_dim + (halves ? (gl < half8 ? gl : gl - half8) * 16 : gl * 8);
+        cs[0] = reinterpret_cast<const float4*>(p)[0];
+        cs[1] = reinterpret_cast<const float4*>(p)[1];
+        if (halves) {
+            cs[2] = reinterpret_cast<const float4*>(p)[2];
+            cs[3] = reinterpret_cast<const float4*>(p)[3];
         }
     }
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = 0.f;
-    if (live) {
-        const char* src = is_q ? a.q + t * a.q_stride : is_k ? a.k + t * a.k_stride : a.v + t * a.v_stride;
-        expand8<A>(load_raw8<A>(src + (static_cast<int64_t>(hk) * D + gl * 8) * AB), f);
+    // where it goes
+    const bool to_cache = kAppend && !is_q;
+    int64_t at = 0;
+    if (to_cache && live) {
+        live = find_slot(a, kv, seq, pos, gl == 0, &at);
+        at += static_cast<int64_t>(h0) * kv.head_stride + gl * 8;
     }
-    const float* w = is_q ? a.q_w : is_k ? a.k_w : nullptr;
-    // the lanes of a group share the branch; the shuffles stay outside it, a
-    // warp may hold groups of either kind
-    float ss = 0.f;
+    char* pool = is_v ? kv.v : kv.k;
+    uint16_t* steps = is_v ? kv.vs : kv.ks;
+    char* dst = (is_q ? a.q_out + t * a.q_out_stride : a.k_out + t * a.k_out_stride) + (h0 * D + gl * 8) * AB;
+    const bool quantises = kAppend && cache == Elem::Q8 && __any_sync(FULL, to_cache && live);
+    const bool normed = a.q_w || a.k_w;
+    const int mate = halves && gl < 2 * half8 ? (gl < half8 ? gl + half8 : gl - half8) : gl;
+    const bool upper = gl >= half8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
+    for (int x = 0; x < HPG; ++x) {
+        float f[8];
+        expand8<A>(raw[x], f);
+        if (normed) {  // for the whole launch: the shuffles stay outside what depends on the head
+            float ss = 0.f;
 #pragma unroll
-    for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
-    if (w) {
-        const float rms = __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(D)), a.eps));
+            for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __fdiv_rn(__fmul_rn(f[i], w[gl * 8 + i]), rms);
-    }
-    const int half8 = a.rope_dim / 16;  // lanes of one half of the rotated elements
-    const int mate = a.pairs == TIR_PAIRS_HALVES && gl < 2 * half8 ? (gl < half8 ? gl + half8 : gl - half8) : gl;
-    float g[8];
+            for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
+            if (w_of) {
+                // one step of Newton's iteration takes rsqrtf's two ulps to one rounding
+                const float v = fmaf(ss, 1.0f / D, a.eps);
+                float inv = rsqrtf(v);
+                if (v >= 1e-30f && v <= 1e30f) inv = fmaf(0.5f * inv, fmaf(-v * inv, inv, 1.0f), inv);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = __shfl_sync(FULL, f[i], mate, G);
-    if (live && turns && gl < 2 * half8) {
-        const float* cs = a.rope + static_cast<int64_t>(pos) * a.rope_dim;
-        if (a.pairs == TIR_PAIRS_ADJACENT) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float c = cs[gl * 8 + 2 * i], s = cs[gl * 8 + 2 * i + 1];
-                const float x = f[2 * i], y = f[2 * i + 1];
-                f[2 * i] = __fadd_rn(__fmul_rn(c, x), __fmul_rn(-s, y));
-                f[2 * i + 1] = __fadd_rn(__fmul_rn(s, x), __fmul_rn(c, y));
+                for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(__fmul_rn(f[i], (&w[i >> 2].x)[i & 3]), inv);
             }
-        } else {
-            const bool upper = gl >= half8;
-            const float* cp = cs + (upper ? gl - half8 : gl) * 16;
+        }
+        if (a.rope && !halves) {
+            if (turns) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float c = i & 1 ? cs[i >> 1].z : cs[i >> 1].x, s = i & 1 ? cs[i >> 1].w : cs[i >> 1].y;
+                    const float u = f[2 * i], v = f[2 * i + 1];
+                    f[2 * i] = __fadd_rn(__fmul_rn(c, u), __fmul_rn(-s, v));
+                    f[2 * i + 1] = __fadd_rn(__fmul_rn(s, u), __fmul_rn(c, v));
+                }
+            }
+        } else if (a.rope) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float c = cp[2 * i], s = upper ? cp[2 * i + 1] : -cp[2 * i + 1];
-                f[i] = __fadd_rn(__fmul_rn(c, f[i]), __fmul_rn(s, g[i]));
+                const float other = __shfl_sync(FULL, f[i], mate, G);
+                if (turns) {
+                    const float c = i & 1 ? cs[i >> 1].z : cs[i >> 1].x, s = i & 1 ? cs[i >> 1].w : cs[i >> 1].y;
+                    f[i] = __fadd_rn(__fmul_rn(c, f[i]), __fmul_rn(upper ? s : -s, other));
+                }
             }
         }
-    }
-    if (kAppend) {
-        const bool write = live && !is_q;
-        store_cache8(f, write, cache, is_k ? kv.k : kv.v, is_k ? kv.ks : kv.vs, at, gl);
-    }
-    if (live && (is_q || !kAppend)) {
-        char* dst = is_q ? a.q_out + t * a.q_out_stride : a.k_out + t * a.k_out_stride;
-        store8_as<A>(dst + (static_cast<int64_t>(hk) * D + gl * 8) * AB, f);
+        const bool write = live && x < n;
+        if (quantises) {
+            uint2 q;
+            float step;
+            quantise8(f, gl & 3, &q, &step);
+            if (write && to_cache) {
+                const int64_t here = at + x * kv.head_stride;
+                *reinterpret_cast<uint2*>(pool + here) = q;
+                if ((gl & 3) == 0) steps[here >> 5] = __half_as_ushort(__float2half_rn(step));
+            }
+        }
+        if (!write) continue;
+        if (!to_cache) {
+            store8_as<A>(dst + x * D * AB, f);
+        } else if (cache != Elem::Q8) {
+            const int64_t here = at + x * kv.head_stride;
+            if (cache == Elem::F32)
+                store8_as<Elem::F32>(pool + here * 4, f);
+            else if (cache == Elem::F16)
+                store8_as<Elem::F16>(pool + here * 2, f);
+            else
+                store8_as<Elem::BF16>(pool + here * 2, f);
+        }
     }
 }
 
-// Group of D / 8 lanes per (token, key or value, head): cache -> rows.
-template <Elem A, int D>
+// Cache -> rows: a group of D / 8 lanes takes HPG of a token's keys and values
+// (HPG = 4 with many tokens: the three lookups before the data are then paid once
+// for four loads in flight).
+template <Elem A, int D, int HPG>
 __global__ void __launch_bounds__(kRowThreads) gather_kernel(const RowArgs a, const PagesView kv, const Elem cache) {
     constexpr int G = D / 8;
     constexpr int AB = ElemOf<A>::bytes;
     const int gl = threadIdx.x % G;
-    const int64_t item = (blockIdx.x * static_cast<int64_t>(kRowThreads) + threadIdx.x) / G;
-    const int64_t t = item / a.heads;
+    const uint32_t item = (blockIdx.x * static_cast<uint32_t>(kRowThreads) + threadIdx.x) / G;
+    const uint32_t t = item / a.chunks;
+    int chunk = static_cast<int>(item % a.chunks);
     if (t >= a.tokens) return;
-    const int h = static_cast<int>(item % a.heads);
-    const bool is_k = h < a.kv_heads;
-    const int hk = is_k ? h : h - a.kv_heads;
+    const bool is_v = chunk >= a.kv_chunks;
+    if (is_v) chunk -= a.kv_chunks;
+    const int h0 = chunk * HPG, n = min(a.kv_heads - h0, HPG);
     const int32_t pos = a.positions[t];
-    if (pos < 0) return;
-    const int64_t row = a.seqs ? a.seqs[t] : t;
-    const int64_t cap = static_cast<int64_t>(kv.max_pages) * kv.page_size;
-    if (row < 0 || row >= kv.table_rows || pos >= cap) {
-        if (gl == 0) atomicOr(a.err, kBadPosition);
-        return;
+    const int32_t seq = a.seqs ? a.seqs[t] : static_cast<int32_t>(t);
+    int64_t at;
+    if (pos < 0 || !find_slot(a, kv, seq, pos, gl == 0, &at)) return;
+    at += static_cast<int64_t>(h0) * kv.head_stride + gl * 8;
+    const char* pool = is_v ? kv.v : kv.k;
+    const uint16_t* steps = is_v ? kv.vs : kv.ks;
+    Raw8<Elem::F32> raw[HPG];
+    float step[HPG];
+#pragma unroll
+    for (int x = 0; x < HPG; ++x) {
+        if (x >= n) break;
+        const int64_t here = at + x * kv.head_stride;
+        if (cache == Elem::Q8) {
+            const uint2 q = *reinterpret_cast<const uint2*>(pool + here);
+            raw[x].w[0].x = q.x, raw[x].w[0].y = q.y;
+            step[x] = __half2float(__ushort_as_half(steps[here >> 5]));
+        } else if (cache == Elem::F32) {
+            raw[x] = load_raw8<Elem::F32>(pool + here * 4);
+        } else {
+            raw[x].w[0] = *reinterpret_cast<const uint4*>(pool + here * 2);
+        }
     }
-    const int32_t id = page_of(kv, row, pos);
-    if (id < 0) return;
-    const int64_t at = slot_of(kv, id, pos) + hk * kv.head_stride + gl * 8;
-    const char* pool = is_k ? kv.k : kv.v;
-    float f[8];
-    if (cache == Elem::Q8) {
-        const uint2 w = *reinterpret_cast<const uint2*>(pool + at);
-        const float step = __half2float(__ushort_as_half((is_k ? kv.ks : kv.vs)[at >> 5]));
-        expand_q8x4(w.x, step, f);
-        expand_q8x4(w.y, step, f + 4);
-    } else if (cache == Elem::F32) {
-        expand8<Elem::F32>(load_raw8<Elem::F32>(pool + at * 4), f);
-    } else if (cache == Elem::F16) {
-        expand8<Elem::F16>(load_raw8<Elem::F16>(pool + at * 2), f);
-    } else {
-        expand8<Elem::BF16>(load_raw8<Elem::BF16>(pool + at * 2), f);
+    char* dst = (is_v ? a.k_out + t * a.k_out_stride : a.q_out + t * a.q_out_stride) + (h0 * D + gl * 8) * AB;
+#pragma unroll
+    for (int x = 0; x < HPG; ++x) {
+        if (x >= n) break;
+        float f[8];
+        if (cache == Elem::Q8) {
+            expand_q8x4(raw[x].w[0].x, step[x], f);
+            expand_q8x4(raw[x].w[0].y, step[x], f + 4);
+        } else if (cache == Elem::F32) {
+            expand8<Elem::F32>(raw[x], f);
+        } else if (cache == Elem::F16) {
+            expand8<Elem::F16>(Raw8<Elem::F16>{{raw[x].w[0]}}, f);
+        } else {
+            expand8<Elem::BF16>(Raw8<Elem::BF16>{{raw[x].w[0]}}, f);
+        }
+        store8_as<A>(dst + x * D * AB, f);
     }
-    char* dst = is_k ? a.q_out + t * a.q_out_stride : a.k_out + t * a.k_out_stride;
-    store8_as<A>(dst + (static_cast<int64_t>(hk) * D + gl * 8) * AB, f);
 }
 
 template <typename F>
@@ -242,21 +331,35 @@ cudaError_t by_type(Elem e, int32_t dim, F&& f) {
     return dims(integral_constant<Elem, Elem::BF16>{});
 }
 
-bool grid_of(const RowArgs& a, int32_t dim, unsigned* grid) {
+// Heads a group of lanes takes, and the grid: four once one each would fill the
+// GPU several times over (8192 tokens of 40 heads of 64 in f32: 35 us with one, 26 with
+// four; 64 tokens: 3.8 and 4.4).
+struct RowShape {
+    bool four;
+    unsigned grid;
+};
+
+bool row_shape(RowArgs* a, int32_t dim, RowShape* s) {
     const int64_t per = kRowThreads / (dim / 8);
-    const int64_t n = (a.tokens * a.heads + per - 1) / per;
-    *grid = static_cast<unsigned>(n);
-    return n <= INT32_MAX;
+    s->four = a->tokens * (a->q_heads + static_cast<int64_t>(a->kinds) * a->kv_heads) > 4 * per * 148 * 8;
+    const int64_t hpg = s->four ? 4 : 1;
+    a->q_chunks = static_cast<int32_t>((a->q_heads + hpg - 1) / hpg);
+    a->kv_chunks = static_cast<int32_t>((a->kv_heads + hpg - 1) / hpg);
+    a->chunks = static_cast<uint32_t>(a->q_chunks + a->kinds * a->kv_chunks);
+    const int64_t items = a->tokens * a->chunks;
+    s->grid = static_cast<unsigned>((items + per - 1) / per);
+    return a->tokens <= INT32_MAX && items + per < (int64_t{1} << 32) / (dim / 8);
 }
 
 template <bool kAppend>
-tir_status launch_rows(const RowArgs& a, const PagesView& kv, Elem act, Elem cache, int32_t dim, void* stream,
+tir_status launch_rows(RowArgs a, const PagesView& kv, Elem act, Elem cache, int32_t dim, void* stream,
                        const char* entry) {
-    unsigned grid;
-    if (!grid_of(a, dim, &grid)) return fail(TIR_ERR_UNSUPPORTED_SHAPE, std::string(entry) + ": too many tokens");
+    RowShape s;
+    if (!row_shape(&a, dim, &s)) return fail(TIR_ERR_UNSUPPORTED_SHAPE, std::string(entry) + ": too many tokens");
     const cudaError_t e = by_type(act, dim, [&](auto el, auto d) {
-        rows_kernel<decltype(el)::value, decltype(d)::value, kAppend>
-            <<<grid, kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, kv, cache);
+        auto* kernel = s.four ? rows_kernel<decltype(el)::value, decltype(d)::value, kAppend, 4>
+                              : rows_kernel<decltype(el)::value, decltype(d)::value, kAppend, 1>;
+        kernel<<<s.grid, kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, kv, cache);
         return cudaGetLastError();
     });
     return e == cudaSuccess ? TIR_OK : paged_fail(e, entry);
@@ -273,6 +376,8 @@ tir_status check_norm(const tir_qk_norm* n, const int32_t* positions, int32_t di
         if (n->rope_positions <= 0) return fail(TIR_ERR_INVALID_ARG, who + ": empty rotation table");
         if (!positions) return fail(TIR_ERR_INVALID_ARG, who + ": a rotation needs positions");
     }
+    if ((reinterpret_cast<uintptr_t>(n->q_weight) | reinterpret_cast<uintptr_t>(n->k_weight) | reinterpret_cast<uintptr_t>(n->rope)) % 16)
+        return fail(TIR_ERR_INVALID_ARG, who + ": weights and rotation table must be 16-byte aligned");
     if ((n->q_weight || n->k_weight) && !(n->eps >= 0.f))
         return fail(TIR_ERR_INVALID_ARG, who + ": eps must not be negative");
     return TIR_OK;
@@ -461,7 +566,7 @@ tir_status tir_qk_norm_rope(const void* q, int64_t q_stride, const void* k, int6
     a.tokens = tokens;
     a.q_heads = q_heads;
     a.kv_heads = kv_heads;
-    a.heads = q_heads + kv_heads;
+    a.kinds = 1;
     set_norm(&a, norm);
     rc = paged_error_word(&a.err);
     if (rc != TIR_OK) return rc;
@@ -504,7 +609,7 @@ static tir_status append(const char* who, const void* q, int64_t q_stride, const
     a.tokens = tokens;
     a.q_heads = q_heads;
     a.kv_heads = kv->kv_heads;
-    a.heads = q_heads + 2 * kv->kv_heads;
+    a.kinds = 2;
     if (norm) set_norm(&a, norm);
     rc = paged_error_word(&a.err);
     if (rc != TIR_OK) return rc;
@@ -556,15 +661,16 @@ tir_status tir_kv_gather(const tir_kv_pages* kv, void* k_out, int64_t k_out_stri
     a.positions = positions;
     a.tokens = tokens;
     a.kv_heads = kv->kv_heads;
-    a.heads = 2 * kv->kv_heads;
+    a.kinds = 2;
     rc = paged_error_word(&a.err);
     if (rc != TIR_OK) return rc;
     view.err = a.err;
-    unsigned grid;
-    if (!grid_of(a, kv->dim, &grid)) return fail(TIR_ERR_UNSUPPORTED_SHAPE, std::string(who) + ": too many tokens");
+    RowShape s;
+    if (!row_shape(&a, kv->dim, &s)) return fail(TIR_ERR_UNSUPPORTED_SHAPE, std::string(who) + ": too many tokens");
     const cudaError_t e = by_type(act, kv->dim, [&](auto el, auto d) {
-        gather_kernel<decltype(el)::value, decltype(d)::value>
-            <<<grid, kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, view, cache);
+        auto* kernel = s.four ? gather_kernel<decltype(el)::value, decltype(d)::value, 4>
+                              : gather_kernel<decltype(el)::value, decltype(d)::value, 1>;
+        kernel<<<s.grid, kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, view, cache);
         return cudaGetLastError();
     });
     return e == cudaSuccess ? TIR_OK : paged_fail(e, who);
