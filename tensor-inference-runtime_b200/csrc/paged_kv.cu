@@ -26,7 +26,7 @@ static __device__ uint32_t g_paged_err;
 namespace {
 
 constexpr uint32_t FULL = 0xffffffffu;
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;
 constexpr int kMaxDevices = 64;
 
 std::mutex g_err_mu;
@@ -130,23 +130,30 @@ __device__ __forceinline__ bool find_slot(const RowArgs& a, const PagesView& kv,
     return true;
 }
 
+enum class Mode { Rows, Fused, FusedQ8, Append, AppendQ8 };
+
+template <int HPG>
+constexpr int kMinBlocks = HPG == 4 ? 6 : 8;
+
 // A group of D / 8 lanes takes HPG heads of one kind (queries, keys or values) of
 // a token.  With many tokens HPG = 4: their loads are in flight together, and the
 // token's position, slot, angles and weights are read once for four heads; with
 // few, HPG = 1 spreads them.  The heads' data are asked for before the slot is
-// looked up.  kAppend: keys and values go to the cache, else keys go to rows and
-// there are no values.
-template <Elem A, int D, bool kAppend, int HPG>
-__global__ void __launch_bounds__(kRowThreads, HPG == 4 ? 3 : 4) rows_kernel(const RowArgs a, const PagesView kv, const Elem cache) {
+// looked up.  M says what a launch does, so that each keeps only the registers it
+// needs (more warps: the kernel is bound by issue and memory alike).
+template <Elem A, int D, Mode M, int HPG>
+__global__ void __launch_bounds__(kRowThreads, kMinBlocks<HPG>) rows_kernel(const RowArgs a, const PagesView kv, const Elem cache) {
     constexpr int G = D / 8;
     constexpr int AB = ElemOf<A>::bytes;
+    constexpr bool kAppend = M != Mode::Rows, kTurn = M == Mode::Rows || M == Mode::Fused || M == Mode::FusedQ8;
+    constexpr bool kQ8 = M == Mode::FusedQ8 || M == Mode::AppendQ8;
     const int gl = threadIdx.x % G;
     const uint32_t item = (blockIdx.x * static_cast<uint32_t>(kRowThreads) + threadIdx.x) / G;
     const uint32_t t = item / a.chunks;
     int chunk = static_cast<int>(item % a.chunks);
-    const bool is_q = chunk < a.q_chunks;
+    const bool is_q = kTurn && chunk < a.q_chunks;
     if (!is_q) chunk -= a.q_chunks;
-    const bool is_v = !is_q && chunk >= a.kv_chunks;
+    const bool is_v = kAppend && !is_q && chunk >= a.kv_chunks;
     if (is_v) chunk -= a.kv_chunks;
     const int h0 = chunk * HPG, n = t < a.tokens ? min((is_q ? a.q_heads : a.kv_heads) - h0, HPG) : 0;
     const int32_t pos = n > 0 && a.positions ? a.positions[t] : 0;
@@ -158,20 +165,20 @@ __global__ void __launch_bounds__(kRowThreads, HPG == 4 ? 3 : 4) rows_kernel(con
         raw[x] = Raw8<A>{};
         if (x < n) raw[x] = load_raw8<A>(src + x * D * AB);
     }
-    const float* w_of = is_q ? a.q_w : is_v ? nullptr : a.k_w;
+    const float* w_of = !kTurn ? nullptr : is_q ? a.q_w : is_v ? nullptr : a.k_w;
     float4 w[2];
     if (w_of) {
         w[0] = reinterpret_cast<const float4*>(w_of)[gl * 2];
         w[1] = reinterpret_cast<const float4*>(w_of)[gl * 2 + 1];
     }
     bool live = n > 0 && pos >= 0;
-    if (live && a.rope && pos >= a.rope_positions) {
+    if (kTurn && live && a.rope && pos >= a.rope_positions) {
         if (gl == 0) atomicOr(a.err, kBadPosition);
         live = false;
     }
     // angles of this lane's elements: four pairs, or with paired halves eight
     const int half8 = a.rope_dim / 16;  // lanes of one half of the rotated elements
-    const bool halves = a.pairs == TIR_PAIRS_HALVES, turns = live && !is_v && gl < 2 * half8;
+    const bool halves = a.pairs == TIR_PAIRS_HALVES, turns = kTurn && live && !is_v && gl < 2 * half8;
     float4 cs[4];
     if (turns) {
         const float* p = a.rope + static_cast<int64_t>(pos) * a.rope_dim + (halves ? (gl < half8 ? gl : gl - half8) * 16 : gl * 8);
@@ -180,6 +187,9 @@ __global__ void __launch_bounds__(kRowThreads, HPG == 4 ? 3 : 4) rows_kernel(con
         if (halves) {
             cs[2] = reinterpret_cast<const float4*>(p)[2];
             cs[3] = reinterpret_cast<const float4*>(p)[3];
+            if (gl < half8)  // the lower half takes the other's element off
+#pragma unroll
+                for (int i = 0; i < 4; ++i) cs[i].y = -cs[i].y, cs[i].w = -cs[i].w;
         }
     }
     // where it goes
@@ -192,10 +202,9 @@ __global__ void __launch_bounds__(kRowThreads, HPG == 4 ? 3 : 4) rows_kernel(con
     char* pool = is_v ? kv.v : kv.k;
     uint16_t* steps = is_v ? kv.vs : kv.ks;
     char* dst = (is_q ? a.q_out + t * a.q_out_stride : a.k_out + t * a.k_out_stride) + (h0 * D + gl * 8) * AB;
-    const bool quantises = kAppend && cache == Elem::Q8 && __any_sync(FULL, to_cache && live);
-    const bool normed = a.q_w || a.k_w;
+    const bool quantises = kQ8 && __any_sync(FULL, to_cache && live);
+    const bool normed = kTurn && (a.q_w || a.k_w);
     const int mate = halves && gl < 2 * half8 ? (gl < half8 ? gl + half8 : gl - half8) : gl;
-    const bool upper = gl >= half8;
 #pragma unroll
     for (int x = 0; x < HPG; ++x) {
         float f[8];
@@ -215,7 +224,7 @@ __global__ void __launch_bounds__(kRowThreads, HPG == 4 ? 3 : 4) rows_kernel(con
                 for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(__fmul_rn(f[i], (&w[i >> 2].x)[i & 3]), inv);
             }
         }
-        if (a.rope && !halves) {
+        if (kTurn && a.rope && !halves) {
             if (turns) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -225,13 +234,13 @@ __global__ void __launch_bounds__(kRowThreads, HPG == 4 ? 3 : 4) rows_kernel(con
                     f[2 * i + 1] = __fadd_rn(__fmul_rn(s, u), __fmul_rn(c, v));
                 }
             }
-        } else if (a.rope) {
+        } else if (kTurn && a.rope) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float other = __shfl_sync(FULL, f[i], mate, G);
                 if (turns) {
                     const float c = i & 1 ? cs[i >> 1].z : cs[i >> 1].x, s = i & 1 ? cs[i >> 1].w : cs[i >> 1].y;
-                    f[i] = __fadd_rn(__fmul_rn(c, f[i]), __fmul_rn(upper ? s : -s, other));
+                    f[i] = fmaf(c, f[i], s * other);
                 }
             }
         }
@@ -249,7 +258,7 @@ __global__ void __launch_bounds__(kRowThreads, HPG == 4 ? 3 : 4) rows_kernel(con
         if (!write) continue;
         if (!to_cache) {
             store8_as<A>(dst + x * D * AB, f);
-        } else if (cache != Elem::Q8) {
+        } else if (!kQ8) {
             const int64_t here = at + x * kv.head_stride;
             if (cache == Elem::F32)
                 store8_as<Elem::F32>(pool + here * 4, f);
@@ -331,9 +340,10 @@ cudaError_t by_type(Elem e, int32_t dim, F&& f) {
     return dims(integral_constant<Elem, Elem::BF16>{});
 }
 
-// Heads a group of lanes takes, and the grid: four once one each would fill the
-// GPU several times over (8192 tokens of 40 heads of 64 in f32: 35 us with one, 26 with
-// four; 64 tokens: 3.8 and 4.4).
+// Heads a group of lanes takes, and the grid: four once one each would give every
+// SM two blocks or more for each of its four schedulers (8192 tokens of 36 heads of
+// 64 in f32: 31.6 us with one, 24.8 with four; 256 tokens of 48 heads of 128 in
+// bf16: 5.7 and 4.1), one below that (64 tokens: 3.1 us).
 struct RowShape {
     bool four;
     unsigned grid;
@@ -341,7 +351,7 @@ struct RowShape {
 
 bool row_shape(RowArgs* a, int32_t dim, RowShape* s) {
     const int64_t per = kRowThreads / (dim / 8);
-    s->four = a->tokens * (a->q_heads + static_cast<int64_t>(a->kinds) * a->kv_heads) > 4 * per * 148 * 8;
+    s->four = a->tokens * (a->q_heads + static_cast<int64_t>(a->kinds) * a->kv_heads) > 4 * per * 148 * 2;
     const int64_t hpg = s->four ? 4 : 1;
     a->q_chunks = static_cast<int32_t>((a->q_heads + hpg - 1) / hpg);
     a->kv_chunks = static_cast<int32_t>((a->kv_heads + hpg - 1) / hpg);
@@ -351,17 +361,30 @@ bool row_shape(RowArgs* a, int32_t dim, RowShape* s) {
     return a->tokens <= INT32_MAX && items + per < (int64_t{1} << 32) / (dim / 8);
 }
 
-template <bool kAppend>
-tir_status launch_rows(RowArgs a, const PagesView& kv, Elem act, Elem cache, int32_t dim, void* stream,
+template <Mode M>
+cudaError_t launch_mode(const RowArgs& a, const PagesView& kv, Elem act, Elem cache, int32_t dim, const RowShape& s, cudaStream_t stream) {
+    return by_type(act, dim, [&](auto el, auto d) {
+        auto* kernel = s.four ? rows_kernel<decltype(el)::value, decltype(d)::value, M, 4>
+                              : rows_kernel<decltype(el)::value, decltype(d)::value, M, 1>;
+        kernel<<<s.grid, kRowThreads, 0, stream>>>(a, kv, cache);
+        return cudaGetLastError();
+    });
+}
+
+// `turned`: norm or rotation on the way (q_heads may be 0).
+tir_status launch_rows(RowArgs a, const PagesView& kv, Elem act, Elem cache, int32_t dim, bool append, bool turned, void* stream,
                        const char* entry) {
     RowShape s;
     if (!row_shape(&a, dim, &s)) return fail(TIR_ERR_UNSUPPORTED_SHAPE, std::string(entry) + ": too many tokens");
-    const cudaError_t e = by_type(act, dim, [&](auto el, auto d) {
-        auto* kernel = s.four ? rows_kernel<decltype(el)::value, decltype(d)::value, kAppend, 4>
-                              : rows_kernel<decltype(el)::value, decltype(d)::value, kAppend, 1>;
-        kernel<<<s.grid, kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, kv, cache);
-        return cudaGetLastError();
-    });
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool q8 = cache == Elem::Q8;
+    cudaError_t e;
+    if (!append)
+        e = launch_mode<Mode::Rows>(a, kv, act, cache, dim, s, st);
+    else if (turned)
+        e = q8 ? launch_mode<Mode::FusedQ8>(a, kv, act, cache, dim, s, st) : launch_mode<Mode::Fused>(a, kv, act, cache, dim, s, st);
+    else
+        e = q8 ? launch_mode<Mode::AppendQ8>(a, kv, act, cache, dim, s, st) : launch_mode<Mode::Append>(a, kv, act, cache, dim, s, st);
     return e == cudaSuccess ? TIR_OK : paged_fail(e, entry);
 }
 
@@ -570,7 +593,7 @@ tir_status tir_qk_norm_rope(const void* q, int64_t q_stride, const void* k, int6
     set_norm(&a, norm);
     rc = paged_error_word(&a.err);
     if (rc != TIR_OK) return rc;
-    return launch_rows<false>(a, PagesView{}, act, Elem::F32, dim, stream, who);
+    return launch_rows(a, PagesView{}, act, Elem::F32, dim, false, true, stream, who);
 }
 
 static tir_status append(const char* who, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
@@ -614,7 +637,7 @@ static tir_status append(const char* who, const void* q, int64_t q_stride, const
     rc = paged_error_word(&a.err);
     if (rc != TIR_OK) return rc;
     view.err = a.err;
-    return launch_rows<true>(a, view, act, cache, kv->dim, stream, who);
+    return launch_rows(a, view, act, cache, kv->dim, true, norm != nullptr, stream, who);
 }
 
 tir_status tir_qk_norm_rope_append(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
