@@ -102,27 +102,32 @@ struct Plan {
     int32_t splits, min_units;
 };
 
-// How many CTAs share a row's head (s).  The time of a call is estimated for rows
-// that are all of the longest length,
-//   waves of (start + a part's units) + join,
-// and for rows spread evenly below it,
-//   all units over the GPU + starts + half a longest part + join,
-// and the s with the least sum of both is taken.  A unit costs a lone CTA kLone,
-// and an SM that holds several of them the time their bytes take (Q8_0: half as
-// much again, its conversions are the bound).  Constants measured on B200:
-// 64 rows x 4 heads x 2048 positions in f32 take 52 us with s = 1, 67 with 2 (a
-// second wave), 59 with 4; 64 rows x 8 heads up to 8192 in bf16 193 us with 1, 171
-// with 4, 205 with 16; one row of 131071 in bf16 1345 us with 1, 91 with 24.
-constexpr double kStart = 3.0, kLone = 0.9, kJoin = 1.5, kJoinRow = 1.0 / 1200.0;  // us
-constexpr double kBytesPerUs = 6.2e6;
+// How many CTAs share a row's head (s).  The time of a call is estimated twice,
+// for rows that are all of the longest length (waves of a start and a part's units)
+// and for rows spread evenly below it (all units over the GPU, starts, half a
+// longest part), and the s with the least sum of the two, each over its least, is
+// taken: the lengths are on the device, and a count that suits both costs either
+// little.  A unit costs a lone CTA kLone, and an SM that holds several the time
+// their bytes take (Q8_0: half as much again, its conversions are the bound).
+// Measured on B200: 64 rows x 4 heads x 2048 positions in f32 take 51 us with s = 1,
+// 57 with 3, 59 with 4; 100 rows x 4 heads up to 6000 161 with 1, 122 with 3, 113 with 6; one
+// row of 131071 in bf16 1332 us with 1, 91 with 37.
+constexpr float kStart = 3.0f, kLone = 0.9f, kJoin = 2.3f, kJoinRow = 1.0f / 1200.0f;  // us
+constexpr float kBytesPerUs = 6.2e6f;
 
-double split_time(int64_t items, int64_t units, int64_t s, int64_t slots, double unit_sm, int sms, int64_t heads) {
+struct SplitTime {
+    float even, ragged;
+};
+
+SplitTime split_time(int64_t items, int64_t units, int64_t s, int64_t slots, float unit_sm, int sms, int64_t heads) {
     const int64_t per = (units + s - 1) / s, parts = (units + per - 1) / per, n = items * parts;
-    auto wave = [&](int64_t ctas) { return kStart + per * std::max(kLone, unit_sm * static_cast<double>(ctas) / sms); };
-    double even = static_cast<double>(n / slots) * wave(slots);
-    if (n % slots) even += wave(n % slots);
-    const double ragged = 0.5 * items * units * unit_sm / sms + kStart * 0.5 * items * (parts + 1) / slots + 0.5 * per * kLone;
-    return even + ragged + (parts > 1 ? 2 * (kJoin + kJoinRow * heads) : 0.0);
+    auto wave = [&](int64_t ctas) { return kStart + per * std::max(kLone, unit_sm * static_cast<float>(ctas) / sms); };
+    const float join = parts > 1 ? kJoin + kJoinRow * heads : 0.f;
+    SplitTime t;
+    t.even = static_cast<float>(n / slots) * wave(slots) + (n % slots ? wave(n % slots) : 0.f) + join;
+    const float all = 0.5f * items * units * unit_sm / sms, longest = kStart + per * kLone;
+    t.ragged = std::max(all + 0.5f * per * kLone, longest) + kStart * 0.35f * items * (parts + 1) / slots + join;
+    return t;
 }
 
 tir_status make_plan(const PagesView& kv, Elem cache, bool f32q, int64_t rows, int32_t q_heads, int64_t max_len,
@@ -139,22 +144,35 @@ tir_status make_plan(const PagesView& kv, Elem cache, bool f32q, int64_t rows, i
     const int64_t units = (n + p->shape.unit - 1) / p->shape.unit;
     const int64_t items = std::max<int64_t>(rows * kv.kv_heads * p->head_tiles, 1);
     const int64_t slots = static_cast<int64_t>(sms) * p->shape.per_sm;
-    const double unit_sm = p->shape.unit * kv.dim * 2.0 * p->shape.bytes * sms / kBytesPerUs;
-    int64_t best = 1;
-    double least = 1e30;
+    const float unit_sm = static_cast<float>(p->shape.unit * kv.dim * 2.0 * p->shape.bytes * sms / kBytesPerUs);
+    int64_t tries[48];
+    SplitTime times[48];
+    int n_tries = 0;
+    float even = 1e30f, ragged = 1e30f;
     auto consider = [&](int64_t s) {
-        const double us = split_time(items, units, s, slots, unit_sm, sms, rows * q_heads);
-        if (us < least) {
-            least = us;
-            best = s;
-        }
+        if (n_tries == 48) return;
+        const SplitTime t = split_time(items, units, s, slots, unit_sm, sms, rows * q_heads);
+        even = std::min(even, t.even);
+        ragged = std::min(ragged, t.ragged);
+        times[n_tries] = t;
+        tries[n_tries++] = s;
     };
-    for (int64_t s = 1; s <= units && (s - 1) * items <= 3 * slots; s += 1 + s / 8) consider(s);
     for (int64_t w = 1; w <= 3; ++w)  // parts that fill whole waves
         if (const int64_t s = w * slots / items; s > 1 && s <= units) consider(s);
+    for (int64_t s = 1; s <= units && (s - 1) * items <= 3 * slots; s += 1 + s / 6) consider(s);
+    int64_t best = 1;
+    float least = 1e30f;
+    for (int i = 0; i < n_tries; ++i) {
+        const float cost = times[i].even / even + (rows > 1 ? times[i].ragged / ragged : 0.f);
+        if (cost < least || (cost == least && tries[i] < best)) {
+            least = cost;
+            best = tries[i];
+        }
+    }
     if (items * best > INT32_MAX) return fail(TIR_ERR_UNSUPPORTED_SHAPE, "tir_paged_attention: too many rows");
     p->splits = static_cast<int32_t>(best);
-    p->min_units = 1;
+    // shorter rows get fewer parts, down to half the length of the longest row's
+    p->min_units = static_cast<int32_t>(std::max<int64_t>((units + best - 1) / best / 2, 1));
     return TIR_OK;
 }
 

@@ -30,6 +30,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -269,11 +270,12 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int tiles = kv.kv_heads * a.head_tiles;
-    const int split = static_cast<int>(blockIdx.x % a.splits);
-    const unsigned rest = blockIdx.x / a.splits;
-    const int64_t row = rest / tiles;
-    const int hk = static_cast<int>(rest % tiles) / a.head_tiles;
-    const int j0 = static_cast<int>(rest % tiles) % a.head_tiles * X::HEADS;  // first head of the group
+    // the heads of a row's part are neighbours: their rows lie side by side in the
+    // pages, and are read at about the same time
+    const int tile = static_cast<int>(blockIdx.x % tiles);
+    const int split = static_cast<int>(blockIdx.x / tiles % a.splits);
+    const int64_t row = blockIdx.x / tiles / a.splits;
+    const int hk = tile / a.head_tiles, j0 = tile % a.head_tiles * X::HEADS;  // key-value head, first head of its group
     const int nh = min(a.group - j0, X::HEADS);
     const int h0 = hk * a.group + j0;
     const int32_t len = row_length(a, kv, row);
@@ -867,7 +869,15 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 template <Elem C, int D, int NT, bool F32Q>
 cudaError_t launch_attn_as(const AttnArgs& a, const PagesView& kv, int64_t rows, cudaStream_t stream) {
     using X = AttnCfg<C, D, NT, F32Q>;
-    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<C, D, NT, F32Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM);
+    // the shared-memory opt-in, once on each device
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = uint64_t{1} << (dev & 63);
+    if (e == cudaSuccess && !(done.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(paged_attn_kernel<C, D, NT, F32Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    }
     if (e != cudaSuccess) return e;
     const unsigned grid = static_cast<unsigned>(rows * kv.kv_heads * a.head_tiles * a.splits);
     paged_attn_kernel<C, D, NT, F32Q><<<grid, X::THREADS, X::SMEM, stream>>>(a, kv);

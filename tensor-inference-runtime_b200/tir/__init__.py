@@ -15,6 +15,7 @@ fails, an exception is raised -- there is no CPU fallback.
 """
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -947,38 +948,34 @@ def rope_table(base, dim, n_pos):
     return out
 
 
+_QK_NORM = struct.Struct("@PPPqiif")  # tir_qk_norm
+
+
 def _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device):
+    """A tir_qk_norm as bytes (ctypes passes their address)."""
     code = PAIRS.get(pairs)
     if code is None:
         raise _bad(f"pairs must be one of {sorted(PAIRS)}")
     t = _torch()
-    n = QKNorm()
-    n.eps = eps
+    table = n_pos = rope_dim = 0
     if rope is not None:
         shape = rope.shape
         if len(shape) != 3 or shape[2] != 2 or rope.dtype is not t.float32 or not rope.is_contiguous():
             raise _bad("rope must be a contiguous float32 [positions, rope_dim / 2, 2] table")
         if rope.get_device() != device:
             raise _bad(f"rope is not on device {device}")
-        n.rope, n.rope_positions, n.rope_dim, n.pairs = rope.data_ptr(), shape[0], 2 * shape[1], code
-    if q_weight is not None:
-        n.q_weight = _weight(q_weight, dim, device, t)
-    if k_weight is not None:
-        n.k_weight = _weight(k_weight, dim, device, t)
-    return n
+        table, n_pos, rope_dim = rope.data_ptr(), shape[0], 2 * shape[1]
+    return _QK_NORM.pack(_weight(q_weight, dim, device, t) if q_weight is not None else 0,
+                         _weight(k_weight, dim, device, t) if k_weight is not None else 0,
+                         table, n_pos, rope_dim, code, eps)
 
 
 def _weight(w, dim, device, t):
-    if w.dim() != 1 or w.shape[0] != dim or w.dtype is not t.float32 or w.stride(0) != 1:
+    if w.shape != (dim,) or w.dtype is not t.float32 or w.stride(0) != 1:
         raise _bad(f"a norm weight must be a contiguous float32 vector of {dim}")
     if w.get_device() != device:
         raise _bad(f"a norm weight is not on device {device}")
     return w.data_ptr()
-
-
-def _same(*counts):
-    if len(set(counts)) != 1:
-        raise _bad("rows of different token counts")
 
 
 def qk_norm_rope(q, k, q_out, k_out, positions, rope=None, q_weight=None, k_weight=None, eps=1e-5, pairs="adjacent",
@@ -996,10 +993,11 @@ def qk_norm_rope(q, k, q_out, k_out, positions, rope=None, q_weight=None, k_weig
     kp, ks, n1 = _rows(k, kh, dim, dtype, device, "k")
     qop, qos, n2 = _rows(q_out, qh, dim, dtype, device, "q_out")
     kop, kos, n3 = _rows(k_out, kh, dim, dtype, device, "k_out")
-    _same(n, n1, n2, n3)
+    if n1 != n or n2 != n or n3 != n:
+        raise _bad("rows of different token counts")
     norm = _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device)
     check(lib().tir_qk_norm_rope(qp, qs, kp, ks, qop, qos, kop, kos, _ints(positions, n, device, "positions"), n, qh, kh,
-                                 dim, code, C.addressof(norm), st))
+                                 dim, code, norm, st))
 
 
 def qk_norm_rope_append(q, k, v, q_out, kv, seqs, positions, rope=None, q_weight=None, k_weight=None, eps=1e-5,
@@ -1015,10 +1013,11 @@ def qk_norm_rope_append(q, k, v, q_out, kv, seqs, positions, rope=None, q_weight
     kp, ks, n1 = _rows(k, kh, dim, dtype, device, "k")
     vp, vs, n2 = _rows(v, kh, dim, dtype, device, "v")
     qop, qos, n3 = _rows(q_out, qh, dim, dtype, device, "q_out")
-    _same(n, n1, n2, n3)
+    if n1 != n or n2 != n or n3 != n:
+        raise _bad("rows of different token counts")
     norm = _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device)
     check(lib().tir_qk_norm_rope_append(qp, qs, kp, ks, vp, vs, qop, qos, kv.ref, _ints(seqs, n, device, "seqs"),
-                                        _ints(positions, n, device, "positions"), n, qh, code, C.addressof(norm), st))
+                                        _ints(positions, n, device, "positions"), n, qh, code, norm, st))
 
 
 def kv_append(kv, k, v, seqs, positions, stream=None):
@@ -1027,7 +1026,8 @@ def kv_append(kv, k, v, seqs, positions, stream=None):
     st = _launch_stream(device, stream)
     kp, ks, n = _rows(k, kv.kv_heads, kv.dim, dtype, device, "k")
     vp, vs, n1 = _rows(v, kv.kv_heads, kv.dim, dtype, device, "v")
-    _same(n, n1)
+    if n1 != n:
+        raise _bad("rows of different token counts")
     check(lib().tir_kv_append(kv.ref, kp, ks, vp, vs, _ints(seqs, n, device, "seqs"),
                               _ints(positions, n, device, "positions"), n, code, st))
 
@@ -1038,7 +1038,8 @@ def kv_gather(kv, k_out, v_out, seqs, positions, stream=None):
     st = _launch_stream(device, stream)
     kp, ks, n = _rows(k_out, kv.kv_heads, kv.dim, dtype, device, "k_out")
     vp, vs, n1 = _rows(v_out, kv.kv_heads, kv.dim, dtype, device, "v_out")
-    _same(n, n1)
+    if n1 != n:
+        raise _bad("rows of different token counts")
     check(lib().tir_kv_gather(kv.ref, kp, ks, vp, vs, _ints(seqs, n, device, "seqs"),
                               _ints(positions, n, device, "positions"), n, code, st))
 
@@ -1064,7 +1065,8 @@ def paged_attention(q, kv, seq_lens, out, scale=0.0, max_len=0, window=0, worksp
     n, qh, _ = q.shape
     qp, qs, _ = _rows(q, qh, kv.dim, dtype, device, "q")
     op, os_, n1 = _rows(out, qh, kv.dim, dtype, device, "out")
-    _same(n, n1)
+    if n1 != n:
+        raise _bad("rows of different token counts")
     size = wp = 0
     if workspace is None:
         size = paged_attention_workspace(kv, n, qh, max_len, window)
