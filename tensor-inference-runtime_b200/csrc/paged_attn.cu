@@ -107,26 +107,25 @@ struct Plan {
 // and for rows spread evenly below it (all units over the GPU, starts, half a
 // longest part), and the s with the least sum of the two, each over its least, is
 // taken: the lengths are on the device, and a count that suits both costs either
-// little.  A unit costs a lone CTA kLone, and an SM that holds several the time
-// their bytes take (Q8_0: half as much again, its conversions are the bound).
+// little.
 // Measured on B200: 64 rows x 4 heads x 2048 positions in f32 take 51 us with s = 1,
 // 57 with 3, 59 with 4; 100 rows x 4 heads up to 6000 161 with 1, 122 with 3, 113 with 6; one
 // row of 131071 in bf16 1332 us with 1, 91 with 37.
-constexpr float kStart = 3.0f, kLone = 0.9f, kJoin = 2.3f, kJoinRow = 1.0f / 1200.0f;  // us
+constexpr float kStart = 3.0f, kJoin = 2.3f, kJoinRow = 1.0f / 1200.0f;  // us
 constexpr float kBytesPerUs = 6.2e6f;
 
 struct SplitTime {
     float even, ragged;
 };
 
-SplitTime split_time(int64_t items, int64_t units, int64_t s, int64_t slots, float unit_sm, int sms, int64_t heads) {
+SplitTime split_time(int64_t items, int64_t units, int64_t s, int64_t slots, float unit_sm, float lone, int sms, int64_t heads) {
     const int64_t per = (units + s - 1) / s, parts = (units + per - 1) / per, n = items * parts;
-    auto wave = [&](int64_t ctas) { return kStart + per * std::max(kLone, unit_sm * static_cast<float>(ctas) / sms); };
+    auto wave = [&](int64_t ctas) { return kStart + per * std::max(lone, unit_sm * static_cast<float>(ctas) / sms); };
     const float join = parts > 1 ? kJoin + kJoinRow * heads : 0.f;
     SplitTime t;
     t.even = static_cast<float>(n / slots) * wave(slots) + (n % slots ? wave(n % slots) : 0.f) + join;
-    const float all = 0.5f * items * units * unit_sm / sms, longest = kStart + per * kLone;
-    t.ragged = std::max(all + 0.5f * per * kLone, longest) + kStart * 0.35f * items * (parts + 1) / slots + join;
+    const float all = 0.5f * items * units * unit_sm / sms, longest = kStart + per * lone;
+    t.ragged = std::max(all + 0.5f * per * lone, longest) + kStart * 0.35f * items * (parts + 1) / slots + join;
     return t;
 }
 
@@ -144,14 +143,14 @@ tir_status make_plan(const PagesView& kv, Elem cache, bool f32q, int64_t rows, i
     const int64_t units = (n + p->shape.unit - 1) / p->shape.unit;
     const int64_t items = std::max<int64_t>(rows * kv.kv_heads * p->head_tiles, 1);
     const int64_t slots = static_cast<int64_t>(sms) * p->shape.per_sm;
-    const float unit_sm = static_cast<float>(p->shape.unit * kv.dim * 2.0 * p->shape.bytes * sms / kBytesPerUs);
+    const float unit_sm = static_cast<float>(p->shape.unit * kv.dim * 2 * p->shape.bytes * sms / kBytesPerUs);
     int64_t tries[48];
     SplitTime times[48];
     int n_tries = 0;
     float even = 1e30f, ragged = 1e30f;
     auto consider = [&](int64_t s) {
         if (n_tries == 48) return;
-        const SplitTime t = split_time(items, units, s, slots, unit_sm, sms, rows * q_heads);
+        const SplitTime t = split_time(items, units, s, slots, unit_sm, p->shape.lone, sms, rows * q_heads);
         even = std::min(even, t.even);
         ragged = std::min(ragged, t.ragged);
         times[n_tries] = t;

@@ -278,6 +278,30 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     const int hk = tile / a.head_tiles, j0 = tile % a.head_tiles * X::HEADS;  // key-value head, first head of its group
     const int nh = min(a.group - j0, X::HEADS);
     const int h0 = hk * a.group + j0;
+    // what depends on no length is asked for along with it: this warp's query heads
+    // (element i * 32 + lane) and, where the row is not divided, its first pages
+    float xq[X::HEADS / X::WARPS][D / 32];
+#pragma unroll
+    for (int y = 0; y < X::HEADS / X::WARPS; ++y)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int j = y * X::WARPS + warp;
+            const int64_t at = row * a.q_stride + static_cast<int64_t>(h0 + j) * D + i * 32 + lane;
+            xq[y][i] = j >= nh                 ? 0.f
+                       : a.act == Elem::F32   ? reinterpret_cast<const float*>(a.q)[at]
+                       : a.act == Elem::F16 ? __half2float(reinterpret_cast<const __half*>(a.q)[at])
+                                            : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.q)[at]);
+        }
+    const bool undivided = a.splits == 1 && a.window == INT32_MAX;
+    int32_t pages[X::AHEAD + 1];
+    if (undivided) {
+        const int32_t cap = kv.max_pages * kv.page_size;
+#pragma unroll
+        for (int i = 0; i <= X::AHEAD; ++i) {
+            const int32_t pos = (i * X::WARPS + warp) * X::TILE + (lane & (X::TILE - 1));
+            pages[i] = pos < cap ? page_id(kv, row, pos) : -1;
+        }
+    }
     const int32_t len = row_length(a, kv, row);
     const AttnRange range = attn_range(len, a.window, a.splits, a.min_units, X::UNIT, split);
     if (range.used == 0) {  // nothing to look at: zeros
@@ -343,9 +367,10 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
             }
         }
     };
-    int32_t pages[X::AHEAD + 1];  // all asked for before the first is waited for
+    if (!undivided) {  // all asked for before the first is waited for
 #pragma unroll
-    for (int i = 0; i <= X::AHEAD; ++i) pages[i] = lookup(i);
+        for (int i = 0; i <= X::AHEAD; ++i) pages[i] = lookup(i);
+    }
 #pragma unroll
     for (int i = 0; i < X::AHEAD; ++i) {
         const uint32_t at = place(i, pages[i]);
@@ -358,18 +383,13 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     int32_t next_page = pages[X::AHEAD];
 
     // ---- q operands, while the first tiles are on their way ----
-    for (int j = warp; j < X::HEADS; j += X::WARPS) {
-        float x[D / 32];
+#pragma unroll
+    for (int y = 0; y < X::HEADS / X::WARPS; ++y) {
+        const int j = y * X::WARPS + warp;
+        float* x = xq[y];
         float top = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
-            x[i] = 0.f;
-            if (j < nh) {
-                const int64_t at = row * a.q_stride + static_cast<int64_t>(h0 + j) * D + i * 32 + lane;
-                x[i] = a.act == Elem::F32   ? reinterpret_cast<const float*>(a.q)[at]
-                       : a.act == Elem::F16 ? __half2float(reinterpret_cast<const __half*>(a.q)[at])
-                                            : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.q)[at]);
-            }
             if constexpr (F32Q) x[i] *= a.scale_log2;
             top = fmaxf(top, fabsf(x[i]));
         }
@@ -884,18 +904,23 @@ cudaError_t launch_attn_as(const AttnArgs& a, const PagesView& kv, int64_t rows,
     return cudaGetLastError();
 }
 
-// Geometry of the kernel that a cache type, head size and query type get: CTAs
-// an SM holds, the positions of a unit, and what an element weighs in bytes.
+// What the split's estimate knows of the kernel that a cache type, head size and
+// query type get: CTAs an SM holds, the positions of a unit, the bytes an element
+// weighs in an SM that holds several (Q8_0: half as much again, its conversions are
+// the bound there), and the time of a unit in a CTA that has an SM to itself
+// (measured on B200: f32 0.93 us with heads of 64 and 1.6 with 128, 16-bit types 0.65
+// with 128 and 1.05 with 256, Q8_0 0.88 with 64 and 1.3 with 128).
 struct AttnShape {
     int per_sm, unit;
-    double bytes;
+    float bytes, lone;
 };
 
 template <Elem C, int D, bool F32Q>
 AttnShape attn_shape_as(int nt) {
-    const double bytes = C == Elem::Q8 ? 1.5 * 34 / 32 : ElemOf<C>::bytes;
-    if (nt == 1) return {AttnCfg<C, D, 1, F32Q>::PER_SM, AttnCfg<C, D, 1, F32Q>::UNIT, bytes};
-    return {AttnCfg<C, D, 2, F32Q>::PER_SM, AttnCfg<C, D, 2, F32Q>::UNIT, bytes};
+    const float bytes = C == Elem::Q8 ? 1.5f * 34 / 32 : ElemOf<C>::bytes;
+    const float each = C == Elem::F32 ? 82e-6f : C == Elem::Q8 ? 32e-6f : 24.5e-6f;  // us an element
+    auto of = [&](auto x) -> AttnShape { return {x.PER_SM, x.UNIT, bytes, 0.25f + each * x.UNIT * 2 * D}; };
+    return nt == 1 ? of(AttnCfg<C, D, 1, F32Q>{}) : of(AttnCfg<C, D, 2, F32Q>{});
 }
 
 // One function per cache type (paged_attn_<type>.cu): the launch, or with `shape`
