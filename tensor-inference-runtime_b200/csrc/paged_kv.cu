@@ -350,6 +350,7 @@ struct RowShape {
 };
 
 bool row_shape(RowArgs* a, int32_t dim, RowShape* s) {
+    if (a->tokens > INT32_MAX) return false;
     const int64_t per = kRowThreads / (dim / 8);
     s->four = a->tokens * (a->q_heads + static_cast<int64_t>(a->kinds) * a->kv_heads) > 4 * per * 148 * 2;
     const int64_t hpg = s->four ? 4 : 1;
@@ -358,7 +359,7 @@ bool row_shape(RowArgs* a, int32_t dim, RowShape* s) {
     a->chunks = static_cast<uint32_t>(a->q_chunks + a->kinds * a->kv_chunks);
     const int64_t items = a->tokens * a->chunks;
     s->grid = static_cast<unsigned>((items + per - 1) / per);
-    return a->tokens <= INT32_MAX && items + per < (int64_t{1} << 32) / (dim / 8);
+    return items + per < (int64_t{1} << 32) / (dim / 8);  // thread numbers are 32-bit
 }
 
 template <Mode M>

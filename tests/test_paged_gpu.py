@@ -184,6 +184,27 @@ def test_attention_pages_and_layouts(cuda, tirlib, act, kind, order, page):
     check_attention(torch, outs[:, 2:8], *attention_ref(torch, q, vals, lens, 0.2, 0), 128, max(lens))
 
 
+@pytest.mark.parametrize("act,kind,dim", [("f32", "f32", 64), ("bf16", "bf16", 128), ("f32", "q8_0", 64), ("f16", "q8_0", 128)])
+def test_attention_many_rows(cuda, tirlib, act, kind, dim):
+    """More rows than the GPU holds CTAs, short and long, a third of them empty; the
+    table longer than the lengths."""
+    torch = cuda
+    rows = 450
+    lens = [(37 * i) % 300 if i % 3 else 0 for i in range(rows)]
+    lens[7] = 1900
+    kv, values, poison = cache(torch, tirlib, kind, rows, 1900, 1, dim, 32, seed=dim)
+    q = torch.randn(rows, 3, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(4)).to(dtype(torch, act))
+    vals = values()
+    poison(lens)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ref = attention_ref(torch, q, vals, lens, 1 / math.sqrt(dim), 0)
+    for max_len in (0, 1900):
+        out = torch.full_like(q, BAD)
+        tirlib.paged_attention(q, kv, n, out, max_len=max_len)
+        check_attention(torch, out, *ref, dim, 1900)
+        assert (out[n == 0] == 0).all()
+
+
 @pytest.mark.parametrize("window", [1, 5, 16, 100, 4000])
 @pytest.mark.parametrize("act,kind", [("f32", "f32"), ("f16", "f16"), ("f32", "q8_0")])
 def test_attention_window(cuda, tirlib, act, kind, window):
@@ -417,6 +438,58 @@ def test_qk_norm_rope(cuda, tirlib, act, pairs, tokens, q_heads, kv_heads, dim, 
     tirlib.ops_check()
 
 
+@pytest.mark.parametrize("tokens,q_heads,kv_heads,dim,rot,pairs", [(1300, 13, 3, 64, 64, "adjacent"), (1300, 13, 3, 64, 32, "halves"),
+                                                                   (901, 9, 5, 128, 48, "halves"), (600, 7, 2, 256, 256, "adjacent")])
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+def test_qk_norm_rope_many_tokens(cuda, tirlib, act, tokens, q_heads, kv_heads, dim, rot, pairs):
+    """Enough heads that a lane group takes four of a kind, the last group fewer."""
+    torch = cuda
+    t = dtype(torch, act)
+    g = torch.Generator("cuda").manual_seed(tokens + dim)
+    row = (3 * torch.randn(tokens, q_heads + kv_heads, dim, device="cuda", generator=g)).to(t)
+    q, k = row[:, :q_heads], row[:, q_heads:]
+    wq, wk = (1 + 0.1 * torch.randn(dim, device="cuda", generator=g) for _ in range(2))
+    table = torch.from_numpy(tirlib.rope_table(10000.0, rot, 700)).cuda()
+    pos = torch.randint(0, 700, (tokens,), device="cuda", generator=g).to(torch.int32)
+    pos[::17] = -1
+    live = pos >= 0
+    q_out, k_out = torch.full((tokens, q_heads, dim), 9.0, dtype=t, device="cuda"), torch.full((tokens, kv_heads, dim), 9.0, dtype=t, device="cuda")
+    tirlib.qk_norm_rope(q, k, q_out, k_out, pos, table, wq, wk, eps=1e-6, pairs=pairs)
+    assert (q_out[~live] == 9.0).all() and (k_out[~live] == 9.0).all()
+    for x, w, out in ((q, wq, q_out), (k, wk, k_out)):
+        ref, mass = norm_rope_ref(torch, x, w, table, pos, pairs, 1e-6)
+        near(torch, out[live], ref[live], mass[live])
+    tirlib.ops_check()
+
+
+def test_qk_norm_rope_without_positions_or_rotation(cuda, tirlib):
+    torch = cuda
+    q, k = torch.randn(7, 4, 64, device="cuda"), torch.randn(7, 2, 64, device="cuda")
+    w = 1 + 0.1 * torch.randn(64, device="cuda")
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    tirlib.qk_norm_rope(q, k, q_out, k_out, None, None, w, w)
+    for x, out in ((q, q_out), (k, k_out)):
+        near(torch, out, *norm_rope_ref(torch, x, w, None, None, "adjacent", 1e-5))
+    tirlib.qk_norm_rope(q, k, q_out, k_out, None)  # nothing to do but copy
+    assert torch.equal(q, q_out) and torch.equal(k, k_out)
+
+
+def test_norm_of_tiny_and_huge_heads(cuda, tirlib):
+    """Sums of squares that leave f32 only where the 64-bit result does, too, and
+    heads of zeros (eps alone under the root)."""
+    torch = cuda
+    x = torch.randn(6, 1, 64, device="cuda")
+    x[0] = 0
+    x[1] *= 1e-18
+    x[2] *= 1e15
+    x[3] *= 1e-4
+    w = torch.ones(64, device="cuda")
+    out, k_out = torch.empty_like(x), torch.empty_like(x)
+    tirlib.qk_norm_rope(x, x, out, k_out, None, None, w, w, eps=1e-5)
+    near(torch, out, *norm_rope_ref(torch, x, w, None, None, "adjacent", 1e-5))
+    assert (out[0] == 0).all()
+
+
 def test_qk_norm_rope_is_the_runtimes_own_rope(cuda, tirlib):
     """Rotation alone, f32, adjacent pairs: bit for bit tir_rope at that position."""
     torch = cuda
@@ -482,6 +555,66 @@ def test_append_and_gather(cuda, tirlib, orc, act, kind, dim, page, kv_heads, or
             y = (y.reshape(*y.shape[:-1], -1, 32) * steps[where].float()[..., None]).reshape(y.shape)
         assert torch.equal(out[ok], y.to(t))
     tirlib.ops_check()
+
+
+@pytest.mark.parametrize("act,kind", [("f32", "q8_0"), ("bf16", "q8_0"), ("f16", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("dim,kv_heads", [(64, 3), (128, 5), (256, 2)])
+def test_append_and_gather_many_tokens(cuda, tirlib, orc, act, kind, dim, kv_heads):
+    """Enough heads that a lane group takes four of a kind; Q8_0 blocks bit for bit."""
+    torch = cuda
+    t, ct = dtype(torch, act), dtype(torch, kind)
+    rows, n, page = 8, 520, 16
+    kv, _, _ = cache(torch, tirlib, kind, rows, n, kv_heads, dim, page, seed=dim)
+    g = torch.Generator("cuda").manual_seed(dim)
+    count = 4000
+    slots = torch.randperm(rows * n, device="cuda", generator=g)[:count]
+    seq, pos = (slots // n).to(torch.int32), (slots % n).to(torch.int32)
+    pos[::29] = -1
+    live = pos >= 0
+    x = (2 * torch.randn(count, 2 * kv_heads, dim, device="cuda", generator=g)).to(t)
+    x[5] = 0
+    k, v = x[:, :kv_heads], x[:, kv_heads:]
+    old = [kv.k.clone(), kv.v.clone()]
+    tirlib.kv_append(kv, k, v, seq, pos)
+    at = (kv.table[seq[live].long(), pos[live].long() // page].long(), pos[live].long() % page)
+    for pool, steps, before, rows_in in ((kv.k, kv.k_scale, old[0], k), (kv.v, kv.v_scale, old[1], v)):
+        if kind == "q8_0":
+            quants, d = q8_blocks(orc, rows_in[live].float().cpu().numpy())
+            before[at] = torch.from_numpy(quants).cuda()
+            assert torch.equal(steps[at].view(torch.int16), torch.from_numpy(d).cuda().view(torch.int16))
+        else:
+            before[at] = rows_in[live].float().to(ct)
+        assert torch.equal(pool, before)
+    out = torch.full((2, count, kv_heads, dim), 4.0, dtype=t, device="cuda")
+    tirlib.kv_gather(kv, out[0], out[1], seq, pos)
+    assert (out[:, ~live] == 4.0).all()
+    for pool, steps, got in ((kv.k, kv.k_scale, out[0]), (kv.v, kv.v_scale, out[1])):
+        y = pool[at].float()
+        if kind == "q8_0":
+            y = (y.reshape(*y.shape[:-1], -1, 32) * steps[at].float()[..., None]).reshape(y.shape)
+        assert torch.equal(got[live], y.to(t))
+    tirlib.ops_check()
+
+
+def test_q8_values_next_to_a_half_step(cuda, tirlib, orc):
+    """Quotients within a few units of the last place of a half, and exact halves:
+    the quants are the divided ones, halves away from zero."""
+    torch = cuda
+    g = torch.Generator("cuda").manual_seed(77)
+    top = 1 + torch.rand(512, 1, 1, device="cuda", generator=g)
+    x = (torch.randint(-126, 126, (512, 1, 64), device="cuda", generator=g) + 0.5) * (top / 127)
+    x = torch.nextafter(x, x + torch.randint(-2, 3, x.shape, device="cuda", generator=g))
+    x[..., ::32] = top                      # sets the step
+    x[256:, :, 7] = 63.5 * 2
+    x[256:, :, 32:] = torch.arange(32, device="cuda") + 0.5
+    x[256:, :, 63] = 127.0                  # step 1: exact halves
+    kv, _, _ = cache(torch, tirlib, "q8_0", 1, 512, 1, 64, 16, seed=2)
+    pos = torch.arange(512, dtype=torch.int32, device="cuda")
+    seq = torch.zeros_like(pos)
+    tirlib.kv_append(kv, x, -x, seq, pos)
+    at = (kv.table[0, pos.long() // 16].long(), pos.long() % 16)
+    for pool, y in ((kv.k, x), (kv.v, -x)):
+        assert torch.equal(pool[at], torch.from_numpy(q8_blocks(orc, y.cpu().numpy())[0]).cuda())
 
 
 def test_q8_blocks_with_infinities_and_nan_stay_apart(cuda, tirlib, orc):
