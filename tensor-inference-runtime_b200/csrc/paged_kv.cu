@@ -136,7 +136,7 @@ template <int HPG>
 constexpr int kMinBlocks = HPG == 4 ? 6 : 8;
 
 // A group of D / 8 lanes takes HPG heads of one kind (queries, keys or values) of
-// a token.  With many tokens HPG = 4: their loads are in flight together, and the
+// a token, a block the same heads of 128 / (D / 8) tokens.  With many tokens HPG = 4: their loads are in flight together, and the
 // token's position, slot, angles and weights are read once for four heads; with
 // few, HPG = 1 spreads them.  The heads' data are asked for before the slot is
 // looked up.  M says what a launch does, so that each keeps only the registers it
@@ -148,9 +148,9 @@ __global__ void __launch_bounds__(kRowThreads, kMinBlocks<HPG>) rows_kernel(cons
     constexpr bool kAppend = M != Mode::Rows, kTurn = M == Mode::Rows || M == Mode::Fused || M == Mode::FusedQ8;
     constexpr bool kQ8 = M == Mode::FusedQ8 || M == Mode::AppendQ8;
     const int gl = threadIdx.x % G;
-    const uint32_t item = (blockIdx.x * static_cast<uint32_t>(kRowThreads) + threadIdx.x) / G;
-    const uint32_t t = item / a.chunks;
-    int chunk = static_cast<int>(item % a.chunks);
+    // a block has one kind of head: what depends on it is the same for all its warps
+    int chunk = static_cast<int>(blockIdx.x % a.chunks);
+    const uint32_t t = blockIdx.x / a.chunks * (kRowThreads / G) + threadIdx.x / G;
     const bool is_q = kTurn && chunk < a.q_chunks;
     if (!is_q) chunk -= a.q_chunks;
     const bool is_v = kAppend && !is_q && chunk >= a.kv_chunks;
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kRowThreads, kMinBlocks<HPG>) rows_kernel(cons
     char* pool = is_v ? kv.v : kv.k;
     uint16_t* steps = is_v ? kv.vs : kv.ks;
     char* dst = (is_q ? a.q_out + t * a.q_out_stride : a.k_out + t * a.k_out_stride) + (h0 * D + gl * 8) * AB;
-    const bool quantises = kQ8 && __any_sync(FULL, to_cache && live);
+    const bool quantises = kQ8 && to_cache && __any_sync(FULL, live);
     const bool normed = kTurn && (a.q_w || a.k_w);
     const int mate = halves && gl < 2 * half8 ? (gl < half8 ? gl + half8 : gl - half8) : gl;
 #pragma unroll
@@ -278,9 +278,8 @@ __global__ void __launch_bounds__(kRowThreads) gather_kernel(const RowArgs a, co
     constexpr int G = D / 8;
     constexpr int AB = ElemOf<A>::bytes;
     const int gl = threadIdx.x % G;
-    const uint32_t item = (blockIdx.x * static_cast<uint32_t>(kRowThreads) + threadIdx.x) / G;
-    const uint32_t t = item / a.chunks;
-    int chunk = static_cast<int>(item % a.chunks);
+    int chunk = static_cast<int>(blockIdx.x % a.chunks);
+    const uint32_t t = blockIdx.x / a.chunks * (kRowThreads / G) + threadIdx.x / G;
     if (t >= a.tokens) return;
     const bool is_v = chunk >= a.kv_chunks;
     if (is_v) chunk -= a.kv_chunks;
@@ -357,9 +356,9 @@ bool row_shape(RowArgs* a, int32_t dim, RowShape* s) {
     a->q_chunks = static_cast<int32_t>((a->q_heads + hpg - 1) / hpg);
     a->kv_chunks = static_cast<int32_t>((a->kv_heads + hpg - 1) / hpg);
     a->chunks = static_cast<uint32_t>(a->q_chunks + a->kinds * a->kv_chunks);
-    const int64_t items = a->tokens * a->chunks;
-    s->grid = static_cast<unsigned>((items + per - 1) / per);
-    return items + per < (int64_t{1} << 32) / (dim / 8);  // thread numbers are 32-bit
+    const int64_t blocks = (a->tokens + per - 1) / per * a->chunks;
+    s->grid = static_cast<unsigned>(blocks);
+    return blocks <= INT32_MAX;
 }
 
 template <Mode M>
