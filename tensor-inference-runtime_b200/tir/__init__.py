@@ -15,7 +15,6 @@ fails, an exception is raised -- there is no CPU fallback.
 """
 import ctypes as C
 import os
-import struct
 
 import numpy as np
 
@@ -823,75 +822,32 @@ def _bad(message):
     return TirError(23, message)  # INVALID_ARG
 
 
-class _Torch:
-    """What the bindings below need of torch on every call, looked up once (torch
-    is imported only by callers that hold tensors)."""
+_bind_module = None
 
-    def __init__(self):
+
+def _bind():
+    """The compiled entry points (bind/paged_bind.cpp): tensor checks and calls."""
+    global _bind_module
+    if _bind_module is None:
         import torch
-        self.codes = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
-        self.float32, self.int32 = torch.float32, torch.int32
-        # the current device and its current stream without the objects around them:
-        # a call's host time is of the order of its kernel's
-        self.device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-        self.stream = getattr(torch._C, "_cuda_getCurrentRawStream",
-                              lambda device: torch.cuda.current_stream(device).cuda_stream)
+        from . import _paged_bind as m
+        addresses = [C.cast(getattr(lib(), "tir_" + n), C.c_void_p).value
+                     for n in ("last_error", "qk_norm_rope", "qk_norm_rope_append", "kv_append", "kv_gather",
+                               "paged_attention", "paged_attention_workspace")]
+        # the current device and its current stream without the objects around them
+        device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda d: torch.cuda.current_stream(d).cuda_stream)
+        m.setup(TirError, device, raw, *addresses)
+        _bind_module = m
+    return _bind_module
 
 
-_torch_state = None
-
-
-def _torch():
-    global _torch_state
-    if _torch_state is None:
-        _torch_state = _Torch()
-    return _torch_state
-
-
-def _rows(x, heads, dim, dtype, device, what):
-    """Checks a [tokens, heads, dim] tensor whose heads are adjacent; returns
-    (pointer, stride between tokens in elements, tokens)."""
-    shape = x.shape
-    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
-        raise _bad(f"{what} must be [tokens, {heads}, {dim}], got {list(shape)}")
-    s0, s1, s2 = x.stride()
-    if s2 != 1 or (s1 != dim and heads > 1):
-        raise _bad(f"{what}: a token's heads must be adjacent")
-    if x.dtype is not dtype:
-        raise _bad(f"{what} has another type than q or k: {x.dtype}")
-    if x.get_device() != device:
-        raise _bad(f"{what} is not on device {device}")
-    n = shape[0]
-    return x.data_ptr(), (s0 if n > 1 else max(s0, heads * dim)), n
-
-
-def _ints(x, n, device, what):
-    """Pointer of a contiguous int32 tensor of at least n values (None: NULL)."""
-    if x is None:
-        return None
-    if x.dim() != 1 or x.dtype is not _torch().int32 or x.shape[0] < n or (n > 1 and x.stride(0) != 1):
-        raise _bad(f"{what} must be a contiguous int32 vector of {n} values")
-    if x.get_device() != device:
-        raise _bad(f"{what} is not on device {device}")
-    return x.data_ptr()
-
-
-def _act(x, what):
-    code = _torch().codes.get(x.dtype)
+def _pairs(pairs):
+    code = PAIRS.get(pairs)
     if code is None:
-        raise TirError(6, f"{what}: activations must be float32, float16 or bfloat16, got {x.dtype}")
+        raise _bad(f"pairs must be one of {sorted(PAIRS)}")
     return code
-
-
-def _launch_stream(device, stream):
-    """The stream to launch on.  The operators run on the current device, and their
-    tensors must be there."""
-    if device < 0:
-        raise _bad("the cache and the activations must be on a CUDA device")
-    t = _torch()
-    if device != t.device():
-        raise _bad(f"the cache or activations are on device {device}, the current device is {t.device()}")
-    return t.stream(device) if stream is None else _stream(stream)
 
 
 class KVPages:
@@ -919,7 +875,9 @@ class KVPages:
                                                 if n > 1):
                     raise _bad("scales must be float16 [n_pages, page_size, kv_heads, dim / 32] in the quants' order")
         else:
-            code = _act(k, "k")
+            code = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}.get(k.dtype)
+            if code is None:
+                raise TirError(6, f"a cache must be float32, float16, bfloat16 or int8, got {k.dtype}")
             if k_scale is not None or v_scale is not None:
                 raise _bad("scales belong to an int8 cache")
         if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
@@ -948,34 +906,8 @@ def rope_table(base, dim, n_pos):
     return out
 
 
-_QK_NORM = struct.Struct("@PPPqiif")  # tir_qk_norm
-
-
-def _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device):
-    """A tir_qk_norm as bytes (ctypes passes their address)."""
-    code = PAIRS.get(pairs)
-    if code is None:
-        raise _bad(f"pairs must be one of {sorted(PAIRS)}")
-    t = _torch()
-    table = n_pos = rope_dim = 0
-    if rope is not None:
-        shape = rope.shape
-        if len(shape) != 3 or shape[2] != 2 or rope.dtype is not t.float32 or not rope.is_contiguous():
-            raise _bad("rope must be a contiguous float32 [positions, rope_dim / 2, 2] table")
-        if rope.get_device() != device:
-            raise _bad(f"rope is not on device {device}")
-        table, n_pos, rope_dim = rope.data_ptr(), shape[0], 2 * shape[1]
-    return _QK_NORM.pack(_weight(q_weight, dim, device, t) if q_weight is not None else 0,
-                         _weight(k_weight, dim, device, t) if k_weight is not None else 0,
-                         table, n_pos, rope_dim, code, eps)
-
-
-def _weight(w, dim, device, t):
-    if w.shape != (dim,) or w.dtype is not t.float32 or w.stride(0) != 1:
-        raise _bad(f"a norm weight must be a contiguous float32 vector of {dim}")
-    if w.get_device() != device:
-        raise _bad(f"a norm weight is not on device {device}")
-    return w.data_ptr()
+def _raw(stream):
+    return None if stream is None else _stream(stream)
 
 
 def qk_norm_rope(q, k, q_out, k_out, positions, rope=None, q_weight=None, k_weight=None, eps=1e-5, pairs="adjacent",
@@ -983,73 +915,30 @@ def qk_norm_rope(q, k, q_out, k_out, positions, rope=None, q_weight=None, k_weig
     """Per-head rmsnorm (where a weight is given) and rotation of q [tokens,
     q_heads, dim] and k [tokens, kv_heads, dim] into q_out and k_out (which may be
     q and k).  positions int32 [tokens]; a negative one leaves its token out."""
-    code, dtype, device = _act(q, "q"), q.dtype, q.get_device()
-    st = _launch_stream(device, stream)
-    if q.dim() != 3 or k.dim() != 3:
-        raise _bad("q and k must be [tokens, heads, dim]")
-    n, qh, dim = q.shape
-    kh = k.shape[1]
-    qp, qs, _ = _rows(q, qh, dim, dtype, device, "q")
-    kp, ks, n1 = _rows(k, kh, dim, dtype, device, "k")
-    qop, qos, n2 = _rows(q_out, qh, dim, dtype, device, "q_out")
-    kop, kos, n3 = _rows(k_out, kh, dim, dtype, device, "k_out")
-    if n1 != n or n2 != n or n3 != n:
-        raise _bad("rows of different token counts")
-    norm = _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device)
-    check(lib().tir_qk_norm_rope(qp, qs, kp, ks, qop, qos, kop, kos, _ints(positions, n, device, "positions"), n, qh, kh,
-                                 dim, code, norm, st))
+    _bind().qk_norm_rope(q, k, q_out, k_out, positions, rope, q_weight, k_weight, eps, _pairs(pairs), _raw(stream))
 
 
 def qk_norm_rope_append(q, k, v, q_out, kv, seqs, positions, rope=None, q_weight=None, k_weight=None, eps=1e-5,
                         pairs="adjacent", stream=None):
     """qk_norm_rope with the keys, and the values as they are, written to the
     cache: token t to position positions[t] of table row seqs[t] (None: row t)."""
-    code, dtype, device, dim, kh = _act(q, "q"), q.dtype, kv.device, kv.dim, kv.kv_heads
-    st = _launch_stream(device, stream)
-    if q.dim() != 3:
-        raise _bad("q must be [tokens, heads, dim]")
-    n, qh, _ = q.shape
-    qp, qs, _ = _rows(q, qh, dim, dtype, device, "q")
-    kp, ks, n1 = _rows(k, kh, dim, dtype, device, "k")
-    vp, vs, n2 = _rows(v, kh, dim, dtype, device, "v")
-    qop, qos, n3 = _rows(q_out, qh, dim, dtype, device, "q_out")
-    if n1 != n or n2 != n or n3 != n:
-        raise _bad("rows of different token counts")
-    norm = _qk_norm(rope, q_weight, k_weight, eps, pairs, dim, device)
-    check(lib().tir_qk_norm_rope_append(qp, qs, kp, ks, vp, vs, qop, qos, kv.ref, _ints(seqs, n, device, "seqs"),
-                                        _ints(positions, n, device, "positions"), n, qh, code, norm, st))
+    _bind().qk_norm_rope_append(q, k, v, q_out, kv.ref, kv.device, seqs, positions, rope, q_weight, k_weight, eps,
+                                _pairs(pairs), _raw(stream))
 
 
 def kv_append(kv, k, v, seqs, positions, stream=None):
     """Rows k, v [tokens, kv_heads, dim] to the cache, rounded or quantised."""
-    code, dtype, device = _act(k, "k"), k.dtype, kv.device
-    st = _launch_stream(device, stream)
-    kp, ks, n = _rows(k, kv.kv_heads, kv.dim, dtype, device, "k")
-    vp, vs, n1 = _rows(v, kv.kv_heads, kv.dim, dtype, device, "v")
-    if n1 != n:
-        raise _bad("rows of different token counts")
-    check(lib().tir_kv_append(kv.ref, kp, ks, vp, vs, _ints(seqs, n, device, "seqs"),
-                              _ints(positions, n, device, "positions"), n, code, st))
+    _bind().kv_append(kv.ref, kv.device, k, v, seqs, positions, _raw(stream))
 
 
 def kv_gather(kv, k_out, v_out, seqs, positions, stream=None):
     """Cached positions back as rows k_out, v_out [tokens, kv_heads, dim]."""
-    code, dtype, device = _act(k_out, "k_out"), k_out.dtype, kv.device
-    st = _launch_stream(device, stream)
-    kp, ks, n = _rows(k_out, kv.kv_heads, kv.dim, dtype, device, "k_out")
-    vp, vs, n1 = _rows(v_out, kv.kv_heads, kv.dim, dtype, device, "v_out")
-    if n1 != n:
-        raise _bad("rows of different token counts")
-    check(lib().tir_kv_gather(kv.ref, kp, ks, vp, vs, _ints(seqs, n, device, "seqs"),
-                              _ints(positions, n, device, "positions"), n, code, st))
+    _bind().kv_gather(kv.ref, kv.device, k_out, v_out, seqs, positions, _raw(stream))
 
 
 def paged_attention_workspace(kv, rows, q_heads, max_len=0, window=0):
     """Bytes of workspace paged_attention needs for these sizes (0: none)."""
-    n = int(lib().tir_paged_attention_workspace(kv.ref, rows, q_heads, max_len, window))
-    if n < 0:
-        raise _bad(lib().tir_last_error().decode(errors="replace"))
-    return n
+    return _bind().workspace(kv.ref, rows, q_heads, max_len, window)
 
 
 def paged_attention(q, kv, seq_lens, out, scale=0.0, max_len=0, window=0, workspace=None, stream=None):
@@ -1058,27 +947,4 @@ def paged_attention(q, kv, seq_lens, out, scale=0.0, max_len=0, window=0, worksp
     zeros for a row of length 0.  workspace: a uint8 tensor of
     paged_attention_workspace bytes; without one it is taken from torch's allocator
     for the call, on the current stream."""
-    code, dtype, device = _act(q, "q"), q.dtype, kv.device
-    st = _launch_stream(device, stream)
-    if q.dim() != 3:
-        raise _bad("q must be [rows, q_heads, dim]")
-    n, qh, _ = q.shape
-    qp, qs, _ = _rows(q, qh, kv.dim, dtype, device, "q")
-    op, os_, n1 = _rows(out, qh, kv.dim, dtype, device, "out")
-    if n1 != n:
-        raise _bad("rows of different token counts")
-    size = wp = 0
-    if workspace is None:
-        size = paged_attention_workspace(kv, n, qh, max_len, window)
-        if size:
-            import torch
-            if st != _torch().stream(device):
-                raise _bad("paged_attention on another stream than the current one needs a workspace")
-            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-            wp = workspace.data_ptr()
-    else:
-        if workspace.get_device() != device or not workspace.is_contiguous():
-            raise _bad(f"workspace must be a contiguous tensor on device {device}")
-        size, wp = workspace.nbytes, workspace.data_ptr()
-    check(lib().tir_paged_attention(qp, qs, kv.ref, _ints(seq_lens, n, device, "seq_lens"), op, os_, n, qh, code, scale,
-                                    max_len, window, wp, size, st))
+    _bind().paged_attention(q, kv.ref, kv.device, seq_lens, out, scale, max_len, window, workspace, _raw(stream))

@@ -6,10 +6,12 @@ the library loads on a machine without a GPU.
 """
 import concurrent.futures
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
@@ -17,6 +19,8 @@ CSRC = os.path.join(ROOT, "csrc")
 INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG_DIR, "libtir.so")
+BIND_SRC = os.path.join(ROOT, "bind", "paged_bind.cpp")
+BIND = os.path.join(PKG_DIR, "_paged_bind.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2,-ffp-contract=off",
@@ -61,12 +65,36 @@ def _compile(src, verbose):
     return obj
 
 
+def build_bind():
+    """Compiles the torch binding of the paged cache operators (needs torch's
+    headers; without torch installed there are no tensors to bind)."""
+    if not _stale(BIND, [BIND_SRC, *_headers(), __file__]):
+        return BIND
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    torch_dir = os.path.dirname(spec.origin)
+    inc = os.path.join(torch_dir, "include")
+    lib = os.path.join(torch_dir, "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-w",
+           "-D_GLIBCXX_USE_CXX11_ABI=1", "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], BIND_SRC, "-o", BIND, "-L" + lib, "-Wl,-rpath," + lib,
+           "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    return BIND
+
+
 def build(verbose=False):
-    """Compiles every CUDA/C++ source and links libtir.so; returns its path."""
+    """Compiles every CUDA/C++ source and links libtir.so (and, with torch
+    installed, its binding of the paged cache operators); returns its path."""
     os.makedirs(BUILD, exist_ok=True)
     srcs = _sources()
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs)) + 1) as ex:
+        bind = ex.submit(build_bind)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
+        bind.result()
     if _stale(LIB, objs):
         cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", LIB, *objs, "-lpthread", "-ldl", "-lrt"]
         r = subprocess.run(cmd, capture_output=True, text=True)
