@@ -107,11 +107,11 @@ struct Plan {
 // and for rows spread evenly below it (all units over the GPU, starts, half a
 // longest part), and the s with the least sum of the two, each over its least, is
 // taken: the lengths are on the device, and a count that suits both costs either
-// little.
-// Measured on B200: 64 rows x 4 heads x 2048 positions in f32 take 51 us with s = 1,
-// 57 with 3, 59 with 4; 100 rows x 4 heads up to 6000 161 with 1, 122 with 3, 113 with 6; one
-// row of 131071 in bf16 1332 us with 1, 91 with 37.
-constexpr float kStart = 3.0f, kJoin = 2.3f, kJoinRow = 1.0f / 1200.0f;  // us
+// little.  Measured on B200: 64 rows x 4 heads x 2048 positions in f32 take 50 us with
+// s = 1, 56 with 3, 60 with 4; 64 rows x 8 heads up to 8192 in bf16 194 with 1, 173 with 4,
+// 189 with 12; one row of 16000 beside 63 of 300 172 with 1, 41 with 6; one row of
+// 131071 1324 with 1, 91 with 37.
+constexpr float kStart = 2.0f, kJoin = 2.3f, kJoinRow = 1.0f / 1200.0f;  // us
 constexpr float kBytesPerUs = 6.2e6f;
 
 struct SplitTime {
@@ -158,7 +158,7 @@ tir_status make_plan(const PagesView& kv, Elem cache, bool f32q, int64_t rows, i
     };
     for (int64_t w = 1; w <= 3; ++w)  // parts that fill whole waves
         if (const int64_t s = w * slots / items; s > 1 && s <= units) consider(s);
-    for (int64_t s = 1; s <= units && (s - 1) * items <= 3 * slots; s += 1 + s / 6) consider(s);
+    for (int64_t s = 1; s <= units && (s - 1) * items <= 8 * slots; s += 1 + s / 6) consider(s);
     int64_t best = 1;
     float least = 1e30f;
     for (int i = 0; i < n_tries; ++i) {
