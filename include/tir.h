@@ -493,10 +493,14 @@ tir_status tir_kv_gather(const tir_kv_pages *kv, void *k_out, int64_t k_out_stri
  * seq_lens is on the device and counts the token itself once it is appended; a
  * row of length 0 gets zeros.  scale multiplies the scores (0: 1 / sqrt(dim)).
  * out has q's type.  f32 queries go with any cache, 16-bit ones with a cache of
- * their own type or Q8_0.  max_len, at least the longest length (0: what the
- * table holds), only sizes the split of long rows over the GPU.  workspace:
- * tir_paged_attention_workspace bytes (0: none is needed, -1: sizes that are
- * refused), 16-byte aligned, of any content, not shared by calls that can run at the same time. */
+ * their own type or Q8_0.  What lies outside a row's positions is never used,
+ * whatever it holds; a NaN or infinity inside makes the head's output
+ * non-finite.  Several query tokens of one sequence are rows of their own, with
+ * the same pages in the table and lengths that end at each.  max_len, at least
+ * the longest length (0: what the table holds), only sizes the split of long
+ * rows over the GPU.  workspace: tir_paged_attention_workspace bytes (0: none
+ * is needed, -1: sizes that are refused), 16-byte aligned, of any content, not
+ * shared by calls that can run at the same time. */
 int64_t tir_paged_attention_workspace(const tir_kv_pages *kv, int64_t rows, int32_t q_heads, int64_t max_len,
                                       int64_t window);
 tir_status tir_paged_attention(const void *q, int64_t q_stride, const tir_kv_pages *kv, const int32_t *seq_lens,

@@ -629,7 +629,8 @@ def test_q8_blocks_with_infinities_and_nan_stay_apart(cuda, tirlib, orc):
     k, v = torch.empty_like(x), torch.empty_like(x)
     tirlib.kv_gather(kv, k, v, seq, pos)
     quants, d = q8_blocks(orc, x.cpu().numpy())
-    want = torch.from_numpy((quants.reshape(4, 4, 32).astype(np.float32) * d.reshape(4, 4, 1).astype(np.float32))).cuda()
+    with np.errstate(invalid="ignore"):  # 0 * inf: the blocks that are spoilt
+        want = torch.from_numpy((quants.reshape(4, 4, 32).astype(np.float32) * d.reshape(4, 4, 1).astype(np.float32))).cuda()
     for got in (k, v):
         got = got.reshape(4, 4, 32)
         assert torch.equal(torch.isfinite(got), torch.isfinite(want))
