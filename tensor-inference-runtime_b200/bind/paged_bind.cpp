@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <exception>
 #include <string>
 
 #include "../../include/tir.h"
@@ -70,7 +71,7 @@ Rows rows(const at::Tensor& x, int64_t heads, int64_t dim, at::ScalarType type, 
     if ((st[2] != 1 && dim > 1) || (st[1] != dim && heads > 1)) bad(std::string(what) + ": a token's heads must be adjacent");
     if (x.scalar_type() != type) bad(std::string(what) + " has another type than q or k: " + c10::toString(x.scalar_type()));
     if (x.get_device() != device) bad(std::string(what) + " is not on device " + std::to_string(device));
-    return {x.data_ptr(), shape[0] > 1 ? st[0] : std::max(st[0], heads * dim), shape[0]};
+    return {x.data_ptr(), shape[0] > 1 ? st[0] : heads * dim, shape[0]};  // one token has no next one
 }
 
 // A contiguous int32 vector of at least n values; None: NULL.
@@ -98,14 +99,20 @@ int64_t integer(PyObject* o) {
     return v;
 }
 
+int32_t integer32(PyObject* o, const char* what) {
+    const int64_t v = integer(o);
+    if (v < 0 || v > INT32_MAX) bad(std::string(what) + " is out of range");
+    return static_cast<int32_t>(v);
+}
+
 double number(PyObject* o) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw Raised();
     return v;
 }
 
-int64_t asked(PyObject* callable, PyObject* arg) {
-    PyObject* r = arg ? PyObject_CallOneArg(callable, arg) : PyObject_CallNoArgs(callable);
+int64_t current_device() {
+    PyObject* r = PyObject_CallNoArgs(S.device);
     if (!r) throw Raised();
     const int64_t v = PyLong_AsLongLong(r);
     Py_DECREF(r);
@@ -113,8 +120,6 @@ int64_t asked(PyObject* callable, PyObject* arg) {
     return v;
 }
 
-// The stream to launch on (None: the current one).  The operators run on the
-// current device, and their tensors must be there.
 int64_t current_stream(int64_t device) {
     PyObject* d = PyLong_FromLongLong(device);
     if (!d) throw Raised();
@@ -127,9 +132,11 @@ int64_t current_stream(int64_t device) {
     return v;
 }
 
+// The stream to launch on (None: the current one).  The operators run on the
+// current device, and their tensors must be there.
 void* stream_of(PyObject* o, int64_t device) {
     if (device < 0) bad("the cache and the activations must be on a CUDA device");
-    const int64_t now = asked(S.device, nullptr);
+    const int64_t now = current_device();
     if (now != device)
         bad("the cache or activations are on device " + std::to_string(device) + ", the current device is " + std::to_string(now));
     return reinterpret_cast<void*>(o == Py_None ? current_stream(device) : integer(o));
@@ -155,7 +162,7 @@ tir_qk_norm norm_of(PyObject* const* a, int64_t dim, int64_t device) {
     n.q_weight = floats(a[1], dim, device);
     n.k_weight = floats(a[2], dim, device);
     n.eps = static_cast<float>(number(a[3]));
-    n.pairs = static_cast<int32_t>(integer(a[4]));
+    n.pairs = integer32(a[4], "pairs");
     return n;
 }
 
@@ -262,12 +269,14 @@ void paged_attention(PyObject* const* a) {
 PyObject* workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
     try {
         if (n != 5) bad("workspace takes 5 arguments");
-        const int64_t b = S.workspace(pages(a[0]), integer(a[1]), static_cast<int32_t>(integer(a[2])), integer(a[3]), integer(a[4]));
+        const int64_t b = S.workspace(pages(a[0]), integer(a[1]), integer32(a[2], "q_heads"), integer(a[3]), integer(a[4]));
         if (b < 0) bad(S.last_error());
         return PyLong_FromLongLong(b);
     } catch (const Raised&) {
-        return nullptr;
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
     }
+    return nullptr;
 }
 
 template <void (*F)(PyObject* const*), int N>
