@@ -5,10 +5,13 @@
 //
 // It is bound by the bytes of the cache, read once: a key-value head's query
 // heads share every key and value.  A CTA takes one (row, key-value head, tile of
-// 8 NT query heads) over a part of the row's positions; its warps take tiles of
-// 16 positions in turn, each with a ring of cp.async stages and a softmax
-// (m, l, o) of its own, so the loop has no CTA barrier.  The parts meet in shared
-// memory, those of different CTAs in paged_attn_join.
+// 8 NT query heads) over a part of the row's positions; its warps take tiles of 16
+// or 32 positions in turn, each with a ring of cp.async half tiles (keys, values,
+// keys, ...) and a softmax (m, l, o) of its own, so the loop has no CTA barrier.
+// The warps' parts meet in shared memory, those of different CTAs in
+// paged_attn_join.  64 rows of 2048 positions take 86 us in bf16 with 8 heads of 128
+// (6.2 TB/s), 50 in f32 with 4 heads of 64 (5.4 TB/s: every value in two tf32 parts)
+// and 24.5 in Q8_0 (2.9 TB/s: bound by the instructions that convert).
 //
 // Products on the tensor cores (mma.sync: with 8 query heads a tile is M = 16
 // positions or dimensions by N = 8 heads, far below the smallest tcgen05 tile,
@@ -20,8 +23,8 @@
 // blocks into the operand layout of P'.
 //
 // Operand types.  K and V enter as they are stored: f16 / bf16 directly, Q8_0
-// quants as f16 integers (exact) with the block steps applied outside, f32 split
-// into two tf32 parts.  q and the weights p are split into as many parts as they
+// quants as exact f16 values (the values' n, the keys' (128 + n) 2^-24) with the
+// block steps applied outside, f32 split into two tf32 parts.  q and the weights p are split into as many parts as they
 // need: 16-bit queries are exact in one (bf16 ones scaled by a power of two for
 // f16), f32 queries take two f16 (22 bits under a per-head power of two), three
 // bf16 or two tf32 parts; p always keeps 16 bits or more (two parts; three bf16
@@ -236,7 +239,9 @@ struct AttnCfg {
     static constexpr int BIAS = q8 ? HEADS * (D / 32) * 4 : 0;
     static constexpr int FIXED = QBYTES + HEADS * 4 + WARPS * HEADS * 8 + BIAS;
     // a warp's ring: SLOTS half tiles (keys, values, keys, ...), an odd number, so that
-    // a step on keys asks for keys.  As many CTAs an SM as three slots each allow.
+    // a step on keys asks for keys.  Three CTAs an SM for heads of 64 (64 x 256 in f32:
+    // 12.5 us, 13.2 with two), two for wider ones where three slots fit (64 x 2048 in
+    // bf16 with heads of 128: 87 us, 95 with three).
     static constexpr int fits(int ctas) { return (227 * 1024 / ctas - 1024 - FIXED) / (WARPS * HALF); }
     static constexpr int PER_SM = fits(3) >= 3 && D == 64 && NT == 1 ? 3 : fits(2) >= 3 ? 2 : 1;
     static constexpr int SLOTS = fits(PER_SM) >= 7 ? 7 : fits(PER_SM) >= 5 ? 5 : 3;

