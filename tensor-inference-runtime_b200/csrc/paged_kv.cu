@@ -4,8 +4,8 @@
 // their pages, and the read-back of cached positions as rows.
 //
 // Every head vector of dim = 64, 128 or 256 elements is held by dim / 8 lanes
-// of one warp, eight elements (one or two 16-byte accesses) each, so the norm's
-// sum, the rotation's partner and a block's maximum are shuffles and every
+// of one warp, eight elements (one or two accesses) each, so the norm's sum and a
+// block's maximum are shuffles, the rotation's partners lie in one lane and every
 // element crosses memory once in and once out: the kernels are bound by memory, and
 // by issue in 16-bit types.
 #include <cuda_runtime.h>
@@ -41,9 +41,7 @@ struct RowArgs {
     int64_t tokens;
     int32_t q_heads, kv_heads;
     int32_t kinds;  // of key-value heads: keys, or keys and values
-    // chunks of a token's heads, none of two kinds: all of them, of queries, of keys
-    uint32_t chunks;
-    int32_t q_chunks, kv_chunks;
+    int32_t q_chunks, kv_chunks;  // chunks of a token's query and key heads
     const float *q_w, *k_w, *rope;
     int64_t rope_positions;
     int32_t rope_dim, pairs;
@@ -57,9 +55,75 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 pair(const float* f, int i) { return make_float2(f[2 * i], f[2 * i + 1]); }
+__device__ __forceinline__ void set_pair(float* f, int i, float2 p) { f[2 * i] = p.x, f[2 * i + 1] = p.y; }
+
+// Eight elements in two runs of four (8-byte aligned in 16-bit types).
+template <Elem E>
+__device__ __forceinline__ Raw8<E> load_raw4x2(const char* p0, const char* p1) {
+    Raw8<E> r;
+    if constexpr (E == Elem::F32) {
+        r.w[0] = *reinterpret_cast<const uint4*>(p0);
+        r.w[1] = *reinterpret_cast<const uint4*>(p1);
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(p0), y = *reinterpret_cast<const uint2*>(p1);
+        r.w[0] = make_uint4(x.x, x.y, y.x, y.y);
+    }
+    return r;
+}
+
+// Rounds and stores them at elements e0 and e1 of p; APART: else e1 = e0 + 4.
+template <Elem E, bool APART>
+__device__ __forceinline__ void store4x2_as(char* p, int e0, int e1, const float* f) {
+    constexpr int B = ElemOf<E>::bytes;
+    if constexpr (!APART) {
+        store8_as<E>(p + e0 * B, f);
+    } else if constexpr (E == Elem::F32) {
+        *reinterpret_cast<float4*>(p + e0 * B) = make_float4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<float4*>(p + e1 * B) = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+        *reinterpret_cast<uint2*>(p + e0 * B) = make_uint2(pack2(f[0], f[1], E), pack2(f[2], f[3], E));
+        *reinterpret_cast<uint2*>(p + e1 * B) = make_uint2(pack2(f[4], f[5], E), pack2(f[6], f[7], E));
+    }
+}
+
 __device__ __forceinline__ float rcp_approx(float x) {  // within one ulp
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ float rsqrt_approx(float x) {
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -76,15 +140,11 @@ __device__ __forceinline__ float rcp_approx(float x) {  // within one ulp
 //   where |x| / |d| >= h - half of f32's step below h, and |x| - h |d| is exact in
 //   one fma (x and h d agree in their leading 13 bits, h d has eight more than d).
 //   Values of 16 bits meet such halves often: x = max / 2 gives 63.5 (dividing there
-//   took 21.4 us for 8192 x 16 heads of 128 in bf16, this takes 18.1);
+//   took 21.4 us for 8192 x 16 heads of 128 in bf16, this took 18.1);
 // * steps too small or too large for either, and NaN, are divided by.
 __device__ __forceinline__ void quantise8(const float* f, int lane4, uint2* quants, float* step) {
-    float hi = f[0], lo = -f[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        hi = max_nan(hi, f[i]);
-        lo = max_nan(lo, -f[i]);
-    }
+    float hi = max3_nan(max3_nan(f[0], f[1], f[2]), max3_nan(f[3], f[4], f[5]), max_nan(f[6], f[7]));
+    float lo = max3_nan(max3_nan(-f[0], -f[1], -f[2]), max3_nan(-f[3], -f[4], -f[5]), max_nan(-f[6], -f[7]));
 #pragma unroll
     for (int w = 1; w <= 2; w <<= 1) {
         hi = max_nan(hi, __shfl_xor_sync(FULL, hi, w));
@@ -106,10 +166,12 @@ __device__ __forceinline__ void quantise8(const float* f, int lane4, uint2* quan
     float far = 0.f;
     constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: a sum with it has the nearest integer in its low bits
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float y = __fmul_rn(f[i], inv), n = __fadd_rn(y, kRound);
-        b[i] = __float_as_uint(n);
-        far = fmaxf(far, fabsf(y - (n - kRound)));
+    for (int i = 0; i < 4; ++i) {
+        const float2 y = mul2(pair(f, i), make_float2(inv, inv)), n = add2(y, make_float2(kRound, kRound));
+        b[2 * i] = __float_as_uint(n.x);
+        b[2 * i + 1] = __float_as_uint(n.y);
+        const float2 off = fma2(add2(n, make_float2(-kRound, -kRound)), make_float2(-1.f, -1.f), y);
+        far = fmaxf(far, fmaxf(fabsf(off.x), fabsf(off.y)));
     }
     if (!(far < 0.5f - 1.0f / 16384.0f)) {
         const float da = fabsf(d), tiny = da * (1.0f / 16777216.0f);
@@ -149,28 +211,37 @@ __device__ __forceinline__ bool find_slot(const RowArgs& a, const PagesView& kv,
 
 enum class Mode { Rows, Fused, FusedQ8, Append, AppendQ8 };
 
-template <int HPG>
-constexpr int kMinBlocks = HPG == 4 ? 6 : 8;
+// Blocks an SM holds: eight of 64 registers a thread where a lane's four heads fit
+// them (4109 tokens of 48 heads of 128 in f16: 22.7 us, with six 23.5; 8 x 1024 tokens
+// of 16 heads of 128 in bf16 to Q8_0 and back: 25.3 and 26.0); where they would spill,
+// six of 80 (norm and rotation of halves only, 8192 tokens of 40 heads of 128 in bf16:
+// 33.9 us, with eight 35.3).
+template <Elem A, Mode M, int HPG, bool H>
+constexpr int kMinBlocks = HPG == 4 && (A == Elem::F32 || M == Mode::FusedQ8 || (M == Mode::Rows && H)) ? 6 : 8;
 
 // A group of D / 8 lanes takes HPG heads of one kind (queries, keys or values) of
 // a token, a block the same heads of 128 / (D / 8) tokens.  With many tokens
 // HPG = 4: their loads are in flight together, and the token's position, slot,
 // angles and weights are read once for four heads; with few, HPG = 1 spreads
 // them.  The heads' data are asked for before the slot is looked up.  M says what
-// a launch does, so that each keeps only the registers it needs (more warps: the
-// kernel is bound by issue and memory alike).  8192 tokens of 36 heads of 64 in f32
-// take 24.8 us (6.1 TB/s), 4109 of 48 heads of 128 in f16 with cache write 26.0
-// (3.9 TB/s).
-template <Elem A, int D, Mode M, int HPG>
-__global__ void __launch_bounds__(kRowThreads, kMinBlocks<HPG>) rows_kernel(const RowArgs a, const PagesView kv, const Elem cache) {
+// a launch does and H that halves are paired in the rotation, so that each keeps
+// only the registers it needs (more warps: the kernel is bound by issue and memory
+// alike).  With paired halves a lane of the rotated part holds four elements of
+// either half, so that it turns pairs of its own with half the angles (with eight
+// consecutive ones and the partners by shuffles 4109 tokens of 48 heads of 128 in
+// f16 took 25.9 us, 64 in bf16 3.0; this takes 21.3 and 2.5); a block to be
+// quantised then goes back to consecutive lanes by as many shuffles.  8192 tokens of
+// 36 heads of 64 in f32 take 24.4 us (6.2 TB/s), the 4109 in f16 run at 4.8 TB/s.
+template <Elem A, int D, Mode M, int HPG, bool H>
+__global__ void __launch_bounds__(kRowThreads, kMinBlocks<A, M, HPG, H>) rows_kernel(const RowArgs a, const PagesView kv, const Elem cache) {
     constexpr int G = D / 8;
     constexpr int AB = ElemOf<A>::bytes;
     constexpr bool kAppend = M != Mode::Rows, kTurn = M == Mode::Rows || M == Mode::Fused || M == Mode::FusedQ8;
     constexpr bool kQ8 = M == Mode::FusedQ8 || M == Mode::AppendQ8;
     const int gl = threadIdx.x % G;
     // a block has one kind of head: what depends on it is the same for all its warps
-    int chunk = static_cast<int>(blockIdx.x % a.chunks);
-    const uint32_t t = blockIdx.x / a.chunks * (kRowThreads / G) + threadIdx.x / G;
+    int chunk = static_cast<int>(blockIdx.x);
+    const uint32_t t = (blockIdx.y + blockIdx.z * gridDim.y) * (kRowThreads / G) + threadIdx.x / G;
     const bool is_q = kTurn && chunk < a.q_chunks;
     if (!is_q) chunk -= a.q_chunks;
     const bool is_v = kAppend && !is_q && chunk >= a.kv_chunks;
@@ -178,74 +249,76 @@ __global__ void __launch_bounds__(kRowThreads, kMinBlocks<HPG>) rows_kernel(cons
     const int h0 = chunk * HPG, n = t < a.tokens ? min((is_q ? a.q_heads : a.kv_heads) - h0, HPG) : 0;
     const int32_t pos = n > 0 && a.positions ? a.positions[t] : 0;
     const int32_t seq = kAppend && n > 0 && a.seqs ? a.seqs[t] : static_cast<int32_t>(t);
-    const char* src = (is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + (h0 * D + gl * 8) * AB;
+    const bool split = H && !is_v && gl < a.rope_dim / 8;
+    const int e0 = split ? gl * 4 : gl * 8, e1 = split ? a.rope_dim / 2 + gl * 4 : gl * 8 + 4;
+    const char* src = (is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + h0 * D * AB;
     Raw8<A> raw[HPG];
 #pragma unroll
     for (int x = 0; x < HPG; ++x) {
         raw[x] = Raw8<A>{};
-        if (x < n) raw[x] = load_raw8<A>(src + x * D * AB);
+        if (x < n) raw[x] = H ? load_raw4x2<A>(src + (x * D + e0) * AB, src + (x * D + e1) * AB) : load_raw8<A>(src + (x * D + e0) * AB);
     }
     const float* w_of = !kTurn ? nullptr : is_q ? a.q_w : is_v ? nullptr : a.k_w;
     float4 w[2];
     if (w_of) {
-        w[0] = reinterpret_cast<const float4*>(w_of)[gl * 2];
-        w[1] = reinterpret_cast<const float4*>(w_of)[gl * 2 + 1];
+        w[0] = *reinterpret_cast<const float4*>(w_of + e0);
+        w[1] = *reinterpret_cast<const float4*>(w_of + e1);
     }
     bool live = n > 0 && pos >= 0;
     if (kTurn && live && a.rope && pos >= a.rope_positions) {
         if (gl == 0) atomicOr(a.err, kBadPosition);
         live = false;
     }
-    // angles of this lane's elements: four pairs, or with paired halves eight
-    const int half8 = a.rope_dim / 16;  // lanes of one half of the rotated elements
-    const bool halves = a.pairs == TIR_PAIRS_HALVES, turns = kTurn && live && !is_v && gl < 2 * half8;
-    float4 cs[4];
+    const bool turns = kTurn && live && !is_v && gl < a.rope_dim / 8;
+    float4 cs[2];  // of this lane's four pairs
     if (turns) {
-        const float* p = a.rope + static_cast<int64_t>(pos) * a.rope_dim + (halves ? (gl < half8 ? gl : gl - half8) * 16 : gl * 8);
+        const float* p = a.rope + static_cast<int64_t>(pos) * a.rope_dim + gl * 8;
         cs[0] = reinterpret_cast<const float4*>(p)[0];
         cs[1] = reinterpret_cast<const float4*>(p)[1];
-        if (halves) {
-            cs[2] = reinterpret_cast<const float4*>(p)[2];
-            cs[3] = reinterpret_cast<const float4*>(p)[3];
-            if (gl < half8)  // the lower half takes the other's element off
-#pragma unroll
-                for (int i = 0; i < 4; ++i) cs[i].y = -cs[i].y, cs[i].w = -cs[i].w;
-        }
     }
     // where it goes
     const bool to_cache = kAppend && !is_q;
     int64_t at = 0;
     if (to_cache && live) {
         live = find_slot(a, kv, seq, pos, gl == 0, &at);
-        at += static_cast<int64_t>(h0) * kv.head_stride + gl * 8;
+        at += static_cast<int64_t>(h0) * kv.head_stride;
     }
     char* pool = is_v ? kv.v : kv.k;
     uint16_t* steps = is_v ? kv.vs : kv.ks;
-    char* dst = (is_q ? a.q_out + t * a.q_out_stride : a.k_out + t * a.k_out_stride) + (h0 * D + gl * 8) * AB;
+    char* dst = (is_q ? a.q_out + t * a.q_out_stride : a.k_out + t * a.k_out_stride) + h0 * D * AB;
     const bool quantises = kQ8 && to_cache && __any_sync(FULL, live);
     const bool normed = kTurn && (a.q_w || a.k_w);
-    const int mate = halves && gl < 2 * half8 ? (gl < half8 ? gl + half8 : gl - half8) : gl;
 #pragma unroll
     for (int x = 0; x < HPG; ++x) {
         float f[8];
         expand8<A>(raw[x], f);
         if (normed) {  // for the whole launch: the shuffles stay outside what depends on the head
-            float ss = 0.f;
+            float2 s2 = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
+            for (int i = 0; i < 4; ++i) s2 = fma2(pair(f, i), pair(f, i), s2);
+            float ss = s2.x + s2.y;
 #pragma unroll
             for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
             if (w_of) {
                 // one step of Newton's iteration takes rsqrtf's two ulps to one rounding
                 const float v = fmaf(ss, 1.0f / D, a.eps);
-                float inv = rsqrtf(v);
-                if (v >= 1e-30f && v <= 1e30f) inv = fmaf(0.5f * inv, fmaf(-v * inv, inv, 1.0f), inv);
+                float inv = rsqrt_approx(v);
+                inv = fmaf(0.5f * inv, fmaf(-v * inv, inv, 1.0f), inv);
+                if (!(v >= 1e-30f && v <= 1e30f)) inv = rsqrtf(v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(__fmul_rn(f[i], (&w[i >> 2].x)[i & 3]), inv);
+                for (int i = 0; i < 4; ++i) set_pair(f, i, mul2(mul2(pair(f, i), pair(&w[i >> 1].x, i & 1)), make_float2(inv, inv)));
             }
         }
-        if (kTurn && a.rope && !halves) {
-            if (turns) {
+        if (turns) {
+            if constexpr (H) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float c = i & 1 ? cs[i >> 1].z : cs[i >> 1].x, s = i & 1 ? cs[i >> 1].w : cs[i >> 1].y;
+                    const float u = f[i], v = f[i + 4];
+                    f[i] = fmaf(c, u, __fmul_rn(-s, v));
+                    f[i + 4] = fmaf(c, v, __fmul_rn(s, u));
+                }
+            } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float c = i & 1 ? cs[i >> 1].z : cs[i >> 1].x, s = i & 1 ? cs[i >> 1].w : cs[i >> 1].y;
@@ -254,38 +327,42 @@ __global__ void __launch_bounds__(kRowThreads, kMinBlocks<HPG>) rows_kernel(cons
                     f[2 * i + 1] = __fadd_rn(__fmul_rn(s, u), __fmul_rn(c, v));
                 }
             }
-        } else if (kTurn && a.rope) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float other = __shfl_sync(FULL, f[i], mate, G);
-                if (turns) {
-                    const float c = i & 1 ? cs[i >> 1].z : cs[i >> 1].x, s = i & 1 ? cs[i >> 1].w : cs[i >> 1].y;
-                    f[i] = fmaf(c, f[i], s * other);
-                }
-            }
         }
         const bool write = live && x < n;
         if (quantises) {
             uint2 q;
             float step;
+            if (H && !is_v) {  // a block's values back to consecutive lanes
+                const bool odd = gl & 1, upper = gl >= a.rope_dim / 16;
+                const int from = 2 * (upper ? gl - a.rope_dim / 16 : gl);
+                const bool swap = split ? upper : odd;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // even lanes send the first half's, then the second's; odd lanes the other way round
+                    const float y = __shfl_sync(FULL, odd ? f[i + 4] : f[i], split ? from + upper : gl, G);
+                    const float z = __shfl_sync(FULL, odd ? f[i] : f[i + 4], split ? from + !upper : gl, G);
+                    f[i] = swap ? z : y;
+                    f[i + 4] = swap ? y : z;
+                }
+            }
             quantise8(f, gl & 3, &q, &step);
             if (write && to_cache) {
-                const int64_t here = at + x * kv.head_stride;
+                const int64_t here = at + x * kv.head_stride + gl * 8;
                 *reinterpret_cast<uint2*>(pool + here) = q;
                 if ((gl & 3) == 0) steps[here >> 5] = __half_as_ushort(__float2half_rn(step));
             }
         }
         if (!write) continue;
         if (!to_cache) {
-            store8_as<A>(dst + x * D * AB, f);
+            store4x2_as<A, H>(dst + x * D * AB, e0, e1, f);
         } else if (!kQ8) {
             const int64_t here = at + x * kv.head_stride;
             if (cache == Elem::F32)
-                store8_as<Elem::F32>(pool + here * 4, f);
+                store4x2_as<Elem::F32, H>(pool + here * 4, e0, e1, f);
             else if (cache == Elem::F16)
-                store8_as<Elem::F16>(pool + here * 2, f);
+                store4x2_as<Elem::F16, H>(pool + here * 2, e0, e1, f);
             else
-                store8_as<Elem::BF16>(pool + here * 2, f);
+                store4x2_as<Elem::BF16, H>(pool + here * 2, e0, e1, f);
         }
     }
 }
@@ -298,8 +375,8 @@ __global__ void __launch_bounds__(kRowThreads) gather_kernel(const RowArgs a, co
     constexpr int G = D / 8;
     constexpr int AB = ElemOf<A>::bytes;
     const int gl = threadIdx.x % G;
-    int chunk = static_cast<int>(blockIdx.x % a.chunks);
-    const uint32_t t = blockIdx.x / a.chunks * (kRowThreads / G) + threadIdx.x / G;
+    int chunk = static_cast<int>(blockIdx.x);
+    const uint32_t t = (blockIdx.y + blockIdx.z * gridDim.y) * (kRowThreads / G) + threadIdx.x / G;
     if (t >= a.tokens) return;
     const bool is_v = chunk >= a.kv_chunks;
     if (is_v) chunk -= a.kv_chunks;
@@ -361,11 +438,11 @@ cudaError_t by_type(Elem e, int32_t dim, F&& f) {
 
 // Heads a group of lanes takes, and the grid: four once one each would give every
 // SM two blocks or more for each of its four schedulers (8192 tokens of 36 heads of
-// 64 in f32: 31.6 us with one, 24.8 with four; 256 tokens of 48 heads of 128 in
-// bf16: 5.7 and 4.1), one below that (64 tokens: 3.1 us).
+// 64 in f32: 31.6 us with one, 24.4 with four; 256 tokens of 48 heads of 128 in
+// bf16: 5.7 and 3.8), one below that (64 tokens: 2.5 us).
 struct RowShape {
     bool four;
-    unsigned grid;
+    dim3 grid;  // chunks of one kind of head, blocks of tokens
 };
 
 bool row_shape(RowArgs* a, int32_t dim, RowShape* s) {
@@ -375,17 +452,23 @@ bool row_shape(RowArgs* a, int32_t dim, RowShape* s) {
     const int64_t hpg = s->four ? 4 : 1;
     a->q_chunks = static_cast<int32_t>((a->q_heads + hpg - 1) / hpg);
     a->kv_chunks = static_cast<int32_t>((a->kv_heads + hpg - 1) / hpg);
-    a->chunks = static_cast<uint32_t>(a->q_chunks + a->kinds * a->kv_chunks);
-    const int64_t blocks = (a->tokens + per - 1) / per * a->chunks;
-    s->grid = static_cast<unsigned>(blocks);
-    return blocks <= INT32_MAX;
+    const int64_t chunks = a->q_chunks + a->kinds * static_cast<int64_t>(a->kv_chunks), blocks = (a->tokens + per - 1) / per;
+    constexpr int64_t kGridY = 32768;  // the grid's second and third dimension end at 65535
+    s->grid = dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(blocks < kGridY ? blocks : kGridY),
+                   static_cast<unsigned>((blocks + kGridY - 1) / kGridY));
+    return chunks * blocks <= INT32_MAX;
 }
 
 template <Mode M>
 cudaError_t launch_mode(const RowArgs& a, const PagesView& kv, Elem act, Elem cache, int32_t dim, const RowShape& s, cudaStream_t stream) {
     return by_type(act, dim, [&](auto el, auto d) {
-        auto* kernel = s.four ? rows_kernel<decltype(el)::value, decltype(d)::value, M, 4>
-                              : rows_kernel<decltype(el)::value, decltype(d)::value, M, 1>;
+        constexpr bool kTurn = M == Mode::Rows || M == Mode::Fused || M == Mode::FusedQ8;
+        auto* kernel = s.four ? rows_kernel<decltype(el)::value, decltype(d)::value, M, 4, false>
+                              : rows_kernel<decltype(el)::value, decltype(d)::value, M, 1, false>;
+        if constexpr (kTurn)
+            if (a.rope && a.pairs == TIR_PAIRS_HALVES)
+                kernel = s.four ? rows_kernel<decltype(el)::value, decltype(d)::value, M, 4, true>
+                                : rows_kernel<decltype(el)::value, decltype(d)::value, M, 1, true>;
         kernel<<<s.grid, kRowThreads, 0, stream>>>(a, kv, cache);
         return cudaGetLastError();
     });

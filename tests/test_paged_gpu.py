@@ -669,6 +669,38 @@ def test_fused_is_norm_rope_then_append(cuda, tirlib, act, kind, pairs):
         assert a is None or torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dim,rot", [(64, 64), (64, 16), (64, 48), (128, 32), (128, 112), (256, 256), (256, 80)])
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+@pytest.mark.parametrize("tokens,q_heads,kv_heads", [(19, 3, 2), (2500, 7, 5)])
+def test_fused_rotates_part_of_a_head(cuda, tirlib, tokens, q_heads, kv_heads, kind, dim, rot):
+    """Rotations of part of the head, with few tokens (a head a group of lanes) and
+    many (four, the last group not full): the cache holds the same bits as after
+    the separate passes, quantised blocks included."""
+    torch = cuda
+    g = torch.Generator("cuda").manual_seed(dim + rot)
+    kv, _, _ = cache(torch, tirlib, kind, 4, 640, kv_heads, dim, 16, seed=1)
+    slots = torch.randperm(4 * 640, device="cuda", generator=g)[:tokens]
+    seq, pos = (slots // 640).to(torch.int32), (slots % 640).to(torch.int32)
+    q = torch.randn(tokens, q_heads, dim, device="cuda", generator=g)
+    k, v = torch.randn(2, tokens, kv_heads, dim, device="cuda", generator=g)
+    w = 1 + 0.1 * torch.randn(2, dim, device="cuda", generator=g)
+    table = torch.from_numpy(tirlib.rope_table(10000.0, rot, 640)).cuda()
+    q_out, q_two = torch.zeros(2, tokens, q_heads, dim, device="cuda")
+    tirlib.qk_norm_rope_append(q, k, v, q_out, kv, seq, pos, table, w[0].contiguous(), w[1].contiguous(), pairs="halves")
+    pools = [y for y in (kv.k, kv.v, kv.k_scale, kv.v_scale) if y is not None]
+    got = [y.clone() for y in pools]
+    for y in pools:
+        y.zero_()
+    k_two = torch.empty_like(k)
+    tirlib.qk_norm_rope(q, k, q_two, k_two, pos, table, w[0].contiguous(), w[1].contiguous(), pairs="halves")
+    tirlib.kv_append(kv, k_two, v, seq, pos)
+    assert torch.equal(q_out, q_two)
+    page, at = kv.table[seq.long(), (pos // 16).long()].long(), (pos % 16).long()
+    for a, b in zip(got, pools):
+        assert torch.equal(a[page, at], b[page, at])
+    tirlib.ops_check()
+
+
 # ---------------------------------------------------------------------------
 # together, as a serving loop uses them
 # ---------------------------------------------------------------------------
