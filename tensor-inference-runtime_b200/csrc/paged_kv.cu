@@ -61,31 +61,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return r;
 }
 
-// Two f32 operations in one instruction.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-    return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 pair(const float* f, int i) { return make_float2(f[2 * i], f[2 * i + 1]); }
-__device__ __forceinline__ void set_pair(float* f, int i, float2 p) { f[2 * i] = p.x, f[2 * i + 1] = p.y; }
-
 // Eight elements in two runs of four (8-byte aligned in 16-bit types).
 template <Elem E>
 __device__ __forceinline__ Raw8<E> load_raw4x2(const char* p0, const char* p1) {
