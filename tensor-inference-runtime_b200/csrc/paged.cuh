@@ -111,6 +111,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
     return r;
 }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, make_float2(-1.f, -1.f), a); }
 __device__ __forceinline__ float2 pair(const float* f, int i) { return make_float2(f[2 * i], f[2 * i + 1]); }
 __device__ __forceinline__ void set_pair(float* f, int i, float2 p) { f[2 * i] = p.x, f[2 * i + 1] = p.y; }
 

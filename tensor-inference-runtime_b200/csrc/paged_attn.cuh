@@ -135,6 +135,14 @@ __device__ __forceinline__ void mma16(float* d, const uint32_t* a, uint32_t b0, 
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// d = c + a b, f16 operands
+__device__ __forceinline__ void mma16_from(float* d, const float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
 // d (16 x 8, f32) += a (16 x 8) b (8 x 8), tf32 operands
 __device__ __forceinline__ void mma8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm(
@@ -493,10 +501,11 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     // c s - base.  The product is rounded (or exact: c is a power of two under f32
     // queries) before the difference is taken, as the maximum's was: equal scores
     // stay equal whatever their size.
-    auto above = [&](float s, int n, int e) -> float {
-        if constexpr (X::plain) return s - base[n][e];
-        else if constexpr (F32Q) return fmaf(s, c[n][e], -base[n][e]);
-        else return __fadd_rn(__fmul_rn(s, c[n][e]), -base[n][e]);
+    auto above = [&](float2 s, int n) -> float2 {
+        const float2 less = make_float2(-base[n][0], -base[n][1]);
+        if constexpr (X::plain) return add2(s, less);
+        else if constexpr (F32Q) return fma2(s, pair(c[n], 0), less);
+        else return add2(mul2(s, pair(c[n], 0)), less);
     };
 
     // ---- the loop over this warp's tiles ----
@@ -549,11 +558,12 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                     const float d0 = k_steps[0].get(b), d1 = k_steps[1].get(b);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        float sum[4] = {off[b][n][0], off[b][n][1], off[b][n][0], off[b][n][1]};
+                        const float from[4] = {off[b][n][0], off[b][n][1], off[b][n][0], off[b][n][1]};
+                        float sum[4];
 #pragma unroll
                         for (int p = X::NQ - 1; p >= 0; --p) {
                             const uint2 q0 = q_op(2 * b, n, p), q1 = q_op(2 * b + 1, n, p);
-                            mma16<false>(sum, x0, q0.x, q0.y);
+                            mma16_from(sum, p == X::NQ - 1 ? from : sum, x0, q0.x, q0.y);
                             mma16<false>(sum, x1, q1.x, q1.y);
                         }
                         s[mt][n][0] = fmaf(sum[0], d0, s[mt][n][0]);
@@ -595,10 +605,12 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                    for (int y = 0; y < 2; ++y) {
                         // smallest parts first
+                        float2 sum = pair(acc[0][n], y);
 #pragma unroll
-                        for (int x = 0; x < CHAINS; ++x) s[mt][n][e] += acc[x][n][e];
+                        for (int x = 1; x < CHAINS; ++x) sum = add2(sum, pair(acc[x][n], y));
+                        set_pair(s[mt][n], y, sum);
                     }
             }
         }
@@ -683,12 +695,14 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         for (int mt = 0; mt < X::MT; ++mt)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
+            {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    s[mt][n][e] = exp2_fast(above(s[mt][n][e], n, e));
-                    s[mt][n][e + 2] = exp2_fast(above(s[mt][n][e + 2], n, e));
-                    l[n][e] += s[mt][n][e] + s[mt][n][e + 2];
+                for (int y = 0; y < 2; ++y) {
+                    const float2 z = above(pair(s[mt][n], y), n);
+                    set_pair(s[mt][n], y, make_float2(exp2_fast(z.x), exp2_fast(z.y)));
                 }
+                set_pair(l[n], 0, add2(pair(l[n], 0), add2(pair(s[mt][n], 0), pair(s[mt][n], 1))));
+            }
 
         // O' += V' P'.  The tensor core's f32 sums are cut off, not rounded: under f32
         // queries a tile's products are summed from zero and then added, so that a
@@ -699,7 +713,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         };
         auto finish = [&](float* sum, const float* acc) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] = F32Q ? sum[e] + acc[e] : acc[e];
+            for (int e = 0; e < 2; ++e) set_pair(sum, e, F32Q ? add2(pair(sum, e), pair(acc, e)) : pair(acc, e));
         };
         if constexpr (X::q8) {
             const float inv = __uint_as_float(static_cast<uint32_t>(127 + 14 - v_exp) << 23);
@@ -717,13 +731,13 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                     uint32_t p0[NT][2], p1[NT][2];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const float w0 = s[mt][n][0] * d0, w1 = s[mt][n][1] * d0, w2 = s[mt][n][2] * d1, w3 = s[mt][n][3] * d1;
-                        const __half2 ha = __floats2half2_rn(w0, w1), hb = __floats2half2_rn(w2, w3);
-                        const float2 fa = __half22float2(ha), fb = __half22float2(hb);
+                        const float2 wa = mul2(pair(s[mt][n], 0), make_float2(d0, d0)), wb = mul2(pair(s[mt][n], 1), make_float2(d1, d1));
+                        const __half2 ha = __float22half2_rn(wa), hb = __float22half2_rn(wb);
+                        const float2 ra = sub2(wa, __half22float2(ha)), rb = sub2(wb, __half22float2(hb));
                         p0[n][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&ha));
                         p0[n][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hb));
-                        p1[n][0] = transpose8x8(pack2(w0 - fa.x, w1 - fa.y, Elem::F16));
-                        p1[n][1] = transpose8x8(pack2(w2 - fb.x, w3 - fb.y, Elem::F16));
+                        p1[n][0] = transpose8x8(pack2(ra.x, ra.y, Elem::F16));
+                        p1[n][1] = transpose8x8(pack2(rb.x, rb.y, Elem::F16));
                     }
                     uint32_t w[4], x[2][4];
                     ldsm4_t(w, v_addr + mt * 16 * X::PITCH + b * 32);
