@@ -132,7 +132,7 @@ __device__ __forceinline__ void expand_q8x4(uint32_t w, float step, float* f) {
 // `row`, and whether it lies in the pool (else the error bit is set).
 __device__ __forceinline__ int32_t page_id(const PagesView& v, int64_t row, int32_t pos) {
     const int32_t i = v.page_shift >= 0 ? pos >> v.page_shift : pos / v.page_size;
-    return __ldg(v.table + row * v.table_stride + i);
+    return v.table[row * v.table_stride + i];
 }
 
 __device__ __forceinline__ bool page_ok(const PagesView& v, int32_t id) {

@@ -38,6 +38,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "launch.cuh"
 #include "paged.cuh"
 #include "ptx.cuh"
 
@@ -53,6 +54,7 @@ struct AttnArgs {
     int32_t splits, min_units;
     float scale_log2;
     Elem act;
+    bool early;  // the launch: may start under the end of the work before it
     float *part_o, *part_ml;  // [rows][q_heads][splits][dim], [..][splits][2]
 };
 
@@ -291,6 +293,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     const int hk = tile / a.head_tiles, j0 = tile % a.head_tiles * X::HEADS;  // key-value head, first head of its group
     const int nh = min(a.group - j0, X::HEADS);
     const int h0 = hk * a.group + j0;
+    griddep_wait();
     // what depends on no length is asked for along with it: this warp's query heads
     // (element i * 32 + lane) and, where the row is not divided, its first pages
     float xq[X::HEADS / X::WARPS][D / 32];
@@ -919,8 +922,7 @@ cudaError_t launch_attn_as(const AttnArgs& a, const PagesView& kv, int64_t rows,
     }
     if (e != cudaSuccess) return e;
     const unsigned grid = static_cast<unsigned>(rows * kv.kv_heads * a.head_tiles * a.splits);
-    paged_attn_kernel<C, D, NT, F32Q><<<grid, X::THREADS, X::SMEM, stream>>>(a, kv);
-    return cudaGetLastError();
+    return launch_kernel(paged_attn_kernel<C, D, NT, F32Q>, dim3(grid), dim3(X::THREADS), X::SMEM, stream, a.early, a, kv);
 }
 
 // What the split's estimate knows of the kernel that a cache type, head size and

@@ -16,6 +16,7 @@
 #include <string>
 #include <vector>
 
+#include "launch.cuh"
 #include "paged.cuh"
 #include "paged.h"
 #include "ptx.cuh"
@@ -222,6 +223,8 @@ __global__ void __launch_bounds__(kRowThreads, kMinBlocks<A, M, HPG, H>) rows_ke
     const bool is_v = kAppend && !is_q && chunk >= a.kv_chunks;
     if (is_v) chunk -= a.kv_chunks;
     const int h0 = chunk * HPG, n = t < a.tokens ? min((is_q ? a.q_heads : a.kv_heads) - h0, HPG) : 0;
+    griddep_launch_dependents();
+    griddep_wait();
     const int32_t pos = n > 0 && a.positions ? a.positions[t] : 0;
     const int32_t seq = kAppend && n > 0 && a.seqs ? a.seqs[t] : static_cast<int32_t>(t);
     const bool split = H && !is_v && gl < a.rope_dim / 8;
@@ -352,6 +355,8 @@ __global__ void __launch_bounds__(kRowThreads) gather_kernel(const RowArgs a, co
     const int gl = threadIdx.x % G;
     int chunk = static_cast<int>(blockIdx.x);
     const uint32_t t = (blockIdx.y + blockIdx.z * gridDim.y) * (kRowThreads / G) + threadIdx.x / G;
+    griddep_launch_dependents();
+    griddep_wait();
     if (t >= a.tokens) return;
     const bool is_v = chunk >= a.kv_chunks;
     if (is_v) chunk -= a.kv_chunks;
@@ -434,6 +439,8 @@ bool row_shape(RowArgs* a, int32_t dim, RowShape* s) {
     return chunks * blocks <= INT32_MAX;
 }
 
+// Both kernels may start under the end of the work before them (64 tokens with cache write:
+// 2.2 us instead of 2.5, 256 3.4 instead of 3.8) and read nothing before it is over.
 template <Mode M>
 cudaError_t launch_mode(const RowArgs& a, const PagesView& kv, Elem act, Elem cache, int32_t dim, const RowShape& s, cudaStream_t stream) {
     return by_type(act, dim, [&](auto el, auto d) {
@@ -444,8 +451,7 @@ cudaError_t launch_mode(const RowArgs& a, const PagesView& kv, Elem act, Elem ca
             if (a.rope && a.pairs == TIR_PAIRS_HALVES)
                 kernel = s.four ? rows_kernel<decltype(el)::value, decltype(d)::value, M, 4, true>
                                 : rows_kernel<decltype(el)::value, decltype(d)::value, M, 1, true>;
-        kernel<<<s.grid, kRowThreads, 0, stream>>>(a, kv, cache);
-        return cudaGetLastError();
+        return launch_kernel(kernel, s.grid, dim3(kRowThreads), 0, stream, true, a, kv, cache);
     });
 }
 
@@ -771,8 +777,7 @@ tir_status tir_kv_gather(const tir_kv_pages* kv, void* k_out, int64_t k_out_stri
     const cudaError_t e = by_type(act, kv->dim, [&](auto el, auto d) {
         auto* kernel = s.four ? gather_kernel<decltype(el)::value, decltype(d)::value, 4>
                               : gather_kernel<decltype(el)::value, decltype(d)::value, 1>;
-        kernel<<<s.grid, kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, view, cache);
-        return cudaGetLastError();
+        return launch_kernel(kernel, s.grid, dim3(kRowThreads), 0, static_cast<cudaStream_t>(stream), true, a, view, cache);
     });
     return e == cudaSuccess ? TIR_OK : paged_fail(e, who);
 }

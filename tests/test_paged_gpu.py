@@ -786,6 +786,63 @@ def test_captured_step_replays_on_new_lengths(cuda, tirlib):
     tirlib.ops_check()
 
 
+@pytest.mark.parametrize("rows,ctx", [(2, 150), (40, 150), (2, 3000)])
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_see_what_was_written_just_before(cuda, tirlib, captured, rows, ctx):
+    """New keys, table and lengths, written by the kernels right before on the same stream
+    and, in a graph, on another one joined to it: the same bits as with waits between."""
+    torch = cuda
+    g = torch.Generator("cuda").manual_seed(rows + ctx)
+    kv, _, _ = cache(torch, tirlib, "bf16", rows, ctx, 2, 64, 16, seed=1)
+    other = torch.cuda.Stream()
+    states = []
+    for i in range(4):
+        table = torch.randperm(kv.table.numel(), device="cuda", generator=g).to(torch.int32).reshape(kv.table.shape)
+        lens = torch.randint(1, ctx + 1, (rows,), device="cuda", generator=g).to(torch.int32)
+        x = torch.randn(rows, 12, 64, device="cuda", generator=g).bfloat16()
+        states.append((table, lens, x))
+    rope = torch.from_numpy(tirlib.rope_table(10000.0, 64, ctx)).cuda()
+    lens, pos, q = torch.zeros(2, rows, dtype=torch.int32, device="cuda").unbind() + (torch.zeros(rows, 8, 64, dtype=torch.bfloat16, device="cuda"),)
+    seq = torch.arange(rows, dtype=torch.int32, device="cuda")
+    ws = torch.empty(max(16, tirlib.paged_attention_workspace(kv, rows, 8, ctx)), dtype=torch.uint8, device="cuda")
+    outs = torch.zeros(2, 24, rows, 8, 64, dtype=torch.bfloat16, device="cuda")
+
+    def step(i, out, wait, fork):
+        table, new, x = states[i % 4]
+        if fork:
+            other.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(other):
+                lens.copy_(new)
+            torch.cuda.current_stream().wait_stream(other)
+        else:
+            lens.copy_(new)
+        kv.table.copy_(table)
+        torch.sub(lens, 1, out=pos)
+        wait()
+        tirlib.qk_norm_rope_append(x[:, :8], x[:, 8:10], x[:, 10:], q, kv, seq, pos, rope)
+        wait()
+        tirlib.paged_attention(q, kv, lens, out, max_len=ctx, workspace=ws)
+        wait()
+
+    before = kv.k.clone(), kv.v.clone()
+    for i in range(24):
+        step(i, outs[0, i], torch.cuda.synchronize, False)
+    kv.k.copy_(before[0])
+    kv.v.copy_(before[1])
+    if captured:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for i in range(24):
+                step(i, outs[1, i], lambda: None, i % 2 == 1)
+        graph.replay()
+    else:
+        for i in range(24):
+            step(i, outs[1, i], lambda: None, False)
+    assert torch.equal(outs[0], outs[1])
+    tirlib.ops_check()
+
+
 def test_streams_run_side_by_side(cuda, tirlib):
     """Two streams, each with its own cache and workspace, many calls in flight."""
     torch = cuda
