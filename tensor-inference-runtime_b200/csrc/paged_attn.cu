@@ -24,7 +24,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join(const AttnArg
     constexpr int N = D / 32;
     __shared__ float part[kJoinWarps][D];
     __shared__ float sums[kJoinWarps];
-    griddep_launch_dependents();
     griddep_wait();
     const int64_t row = blockIdx.x / a.q_heads;
     const int h = static_cast<int>(blockIdx.x % a.q_heads);
@@ -259,10 +258,6 @@ tir_status tir_paged_attention(const void* q, int64_t q_stride, const tir_kv_pag
     a.act = act;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + (need > 0 ? rows * q_heads * p.splits * kv->dim : 0);
-    // May start under the end of the work before it only where every CTA finds an SM of its
-    // own: more would gather on the SMs that come free first (1 row of 144 in f32: 5.6 us
-    // instead of 6.0; 64 rows of 2048, 256 CTAs: 56 instead of 49).
-    a.early = p.splits == 1 && rows * kv->kv_heads * p.head_tiles <= multiprocessors();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = attn(&a, view, cache, act == Elem::F32, p.nt, rows, st, nullptr);
     if (e == cudaSuccess && p.splits > 1) {

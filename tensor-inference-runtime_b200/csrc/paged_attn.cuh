@@ -54,7 +54,6 @@ struct AttnArgs {
     int32_t splits, min_units;
     float scale_log2;
     Elem act;
-    bool early;  // the launch: may start under the end of the work before it
     float *part_o, *part_ml;  // [rows][q_heads][splits][dim], [..][splits][2]
 };
 
@@ -838,7 +837,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         }
     }
     cp_async_wait_all();
-    griddep_launch_dependents();
+    if (a.splits > 1) griddep_launch_dependents();  // the join
     __syncwarp();
 
     // ---- the warps' parts joined ----
@@ -922,7 +921,7 @@ cudaError_t launch_attn_as(const AttnArgs& a, const PagesView& kv, int64_t rows,
     }
     if (e != cudaSuccess) return e;
     const unsigned grid = static_cast<unsigned>(rows * kv.kv_heads * a.head_tiles * a.splits);
-    return launch_kernel(paged_attn_kernel<C, D, NT, F32Q>, dim3(grid), dim3(X::THREADS), X::SMEM, stream, a.early, a, kv);
+    return launch_kernel(paged_attn_kernel<C, D, NT, F32Q>, dim3(grid), dim3(X::THREADS), X::SMEM, stream, true, a, kv);
 }
 
 // What the split's estimate knows of the kernel that a cache type, head size and
