@@ -205,9 +205,9 @@ constexpr int kMinBlocks = HPG == 4 && (A == Elem::F32 || M == Mode::FusedQ8 || 
 // alike).  With paired halves a lane of the rotated part holds four elements of
 // either half, so that it turns pairs of its own with half the angles (with eight
 // consecutive ones and the partners by shuffles 4109 tokens of 48 heads of 128 in
-// f16 took 25.9 us, 64 in bf16 3.0; this takes 21.3 and 2.5); a block to be
+// f16 took 25.9 us, 64 in bf16 3.0; this takes 20.8 and 2.3); a block to be
 // quantised then goes back to consecutive lanes by as many shuffles.  8192 tokens of
-// 36 heads of 64 in f32 take 24.4 us (6.2 TB/s), the 4109 in f16 run at 4.8 TB/s.
+// 36 heads of 64 in f32 take 24.4 us (6.2 TB/s), the 4109 in f16 run at 4.9 TB/s.
 template <Elem A, int D, Mode M, int HPG, bool H>
 __global__ void __launch_bounds__(kRowThreads, kMinBlocks<A, M, HPG, H>) rows_kernel(const RowArgs a, const PagesView kv, const Elem cache) {
     constexpr int G = D / 8;
@@ -416,8 +416,8 @@ cudaError_t by_type(Elem e, int32_t dim, F&& f) {
 
 // Heads a group of lanes takes, and the grid: four once one each would give every
 // SM two blocks or more for each of its four schedulers (8192 tokens of 36 heads of
-// 64 in f32: 31.6 us with one, 24.4 with four; 256 tokens of 48 heads of 128 in
-// bf16: 5.7 and 3.8), one below that (64 tokens: 2.5 us).
+// 64 in f32: 31.6 us with one, 24.4 with four; 512 tokens of 48 heads of 128 in
+// bf16: 5.2 and 4.1, 256 3.4 and 3.5), one below that (64 tokens: 2.3 us).
 struct RowShape {
     bool four;
     dim3 grid;  // chunks of one kind of head, blocks of tokens
