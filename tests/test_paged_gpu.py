@@ -843,6 +843,71 @@ def test_calls_see_what_was_written_just_before(cuda, tirlib, captured, rows, ct
     tirlib.ops_check()
 
 
+@pytest.mark.parametrize("before", ["copy", "set", "upload", "event", "nothing"])
+def test_a_graph_of_one_call_behind_any_node(cuda, tirlib, before):
+    """What stands before a call in a graph may be a copy, a memory set, an upload, another
+    stream's work or nothing: the call waits for it."""
+    torch = cuda
+    kv, _, _ = cache(torch, tirlib, "f32", 3, 700, 2, 64, 16, seed=1)
+    q = torch.randn(3, 8, 64, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    want = torch.tensor([700, 1, 333], dtype=torch.int32)
+    if before == "set":
+        want.zero_()
+    host = want.pin_memory()
+    lens, new, out, ref = want.cuda(), want.cuda(), torch.ones_like(q), torch.empty_like(q)
+    ws = torch.empty(max(16, tirlib.paged_attention_workspace(kv, 3, 8, 700)), dtype=torch.uint8, device="cuda")
+    tirlib.paged_attention(q, kv, lens, ref, max_len=700, workspace=ws)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        if before == "copy":
+            lens.copy_(new)
+        elif before == "set":
+            lens.zero_()
+        elif before == "upload":
+            lens.copy_(host, non_blocking=True)
+        elif before == "event":
+            other.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(other):
+                torch.add(new, 0, out=lens)
+            torch.cuda.current_stream().wait_stream(other)
+        tirlib.paged_attention(q, kv, lens, out, max_len=700, workspace=ws)
+    for _ in range(3):
+        if before != "nothing":
+            lens.fill_(5)
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref)
+    tirlib.ops_check()
+
+
+def test_more_blocks_of_tokens_than_one_dimension_of_a_grid(cuda, tirlib):
+    """140001 tokens of one head of 256: 35001 blocks."""
+    torch = cuda
+    n, dim, page = 140001, 256, 64
+    g = torch.Generator("cuda").manual_seed(5)
+    q, k = torch.randn(2, n, 1, dim, device="cuda", generator=g).bfloat16()
+    w = 1 + 0.1 * torch.randn(dim, device="cuda", generator=g)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    tirlib.qk_norm_rope(q, k, q_out, k_out, pos, None, w, w, eps=1e-6)
+    for x, out in ((q, q_out), (k, k_out)):
+        ref, mass = norm_rope_ref(torch, x, w, None, pos, "halves", 1e-6)
+        near(torch, out, ref, mass)
+    pages = -(-n // page)
+    pool = torch.zeros(2, pages, page, 1, dim, dtype=torch.bfloat16, device="cuda")
+    table = torch.randperm(pages, device="cuda", generator=g).to(torch.int32).reshape(1, pages)
+    kv = tirlib.KVPages(pool[0], pool[1], table)
+    seq = torch.zeros(n, dtype=torch.int32, device="cuda")
+    tirlib.kv_append(kv, k_out, q_out, seq, pos)
+    back = torch.zeros(2, n, 1, dim, dtype=torch.bfloat16, device="cuda")
+    tirlib.kv_gather(kv, back[0], back[1], seq, pos)
+    assert torch.equal(back[0], k_out) and torch.equal(back[1], q_out)
+    tirlib.ops_check()
+
+
 def test_streams_run_side_by_side(cuda, tirlib):
     """Two streams, each with its own cache and workspace, many calls in flight."""
     torch = cuda
