@@ -155,7 +155,8 @@ __device__ __forceinline__ void quantise8(const float* f, int lane4, uint2* quan
         for (int i = 0; i < 8; ++i) {
             const float n = __fadd_rd(fabsf(__fmul_rn(f[i], inv)), 8388608.0f);  // 2^23 + floor
             const float h = n - 8388607.5f;
-            const float half = __uint_as_float(__float_as_uint(h) & 0x7f800000u) * tiny;  // half a step below h, times |d|
+            // half a step below h, times |d|: the step is that of the value just below (h = 1/2 is a power of two)
+            const float half = __uint_as_float((__float_as_uint(h) - 1u) & 0x7f800000u) * tiny;
             const float m = h + (fmaf(-h, da, fabsf(f[i])) >= -half ? 0.5f : -0.5f);
             b[i] = __float_as_uint(copysignf(m, __uint_as_float(__float_as_uint(f[i]) ^ __float_as_uint(d))) + kRound);
         }
