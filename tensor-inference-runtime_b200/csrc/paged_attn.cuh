@@ -27,9 +27,10 @@
 // block steps applied outside, f32 split into two tf32 parts.  q and the weights p are split into as many parts as they
 // need: 16-bit queries are exact in one (bf16 ones scaled by a power of two for
 // f16), f32 queries take two f16 (22 bits under a per-head power of two), three
-// bf16 or two tf32 parts; p always keeps 16 bits or more (two parts; three bf16
-// under f32 queries), below the rounding of the output.  Scores, m, l and o are
-// f32 throughout.
+// bf16 or two tf32 parts.  p has two bf16 parts (16 bits, below the rounding of a
+// 16-bit output; three under f32 queries), two tf32 parts or two f16 ones, the
+// second kept above its place so that f16's range does not cut small weights off.
+// Scores, m, l and o are f32 throughout.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -221,7 +222,7 @@ struct Steps {
 // queries (else 16-bit ones).
 template <Elem C, int D, int NT, bool F32Q>
 struct AttnCfg {
-    static constexpr bool tf32 = C == Elem::F32, bf = C == Elem::BF16, q8 = C == Elem::Q8;
+    static constexpr bool tf32 = C == Elem::F32, f16 = C == Elem::F16, bf = C == Elem::BF16, q8 = C == Elem::Q8;
     static constexpr int ES = ElemOf<C>::bytes;
     static constexpr int NQ = tf32 ? 2 : !F32Q ? 1 : bf ? 3 : 2;  // parts of q
     static constexpr int NP = tf32 ? 2 : bf && F32Q ? 3 : 2;      // parts of p
@@ -271,10 +272,10 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     constexpr uint32_t FULL = 0xffffffffu;
     constexpr int CH = X::ROW / 16;        // 16-byte pieces of a cached row
     constexpr int LPR = CH < 8 ? CH : 8;  // lanes that copy a row
-    // weights are kept 2^6 above their logarithm's reference, and the reference may
-    // lag the maximum by 8: f16 parts then lose nothing to the end of its range
-    constexpr float kLift = X::tf32 || X::bf ? 0.f : 6.f;
-    constexpr float kLag = 8.f;
+    // weights are 2^kLift above their logarithm's reference, which may lag the maximum by
+    // kLag: weights in f16 parts fill its range from the top (2^15)
+    constexpr float kLift = X::f16 ? 11.f : X::q8 ? 6.f : 0.f;
+    constexpr float kLag = X::f16 ? 4.f : 8.f;
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* ring = smem;
     uint32_t* qf = reinterpret_cast<uint32_t*>(smem + X::RING);
@@ -801,27 +802,36 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                 for (int n = 0; n < NT; ++n) finish(o[i][n], acc[n]);
             }
         } else {
+            // f16's second part of a weight is kept 2^12 above its place, in a sum of its own:
+            // in its place its digits would end with f16's range, from weights of 2^-12 of the
+            // reference's on (a key that leads the row by 8), and a long row sums 10^5 of those.
+            // So 20 bits remain down to 2^-28 (19), 12 to 2^-36 (25).
+            constexpr float kRest = 4096.f;
             uint32_t pp[X::MT][NT][X::NP][2];
 #pragma unroll
             for (int mt = 0; mt < X::MT; ++mt)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float r0 = s[mt][n][0], r1 = s[mt][n][1], r2 = s[mt][n][2], r3 = s[mt][n][3];
+                    float2 ra = pair(s[mt][n], 0), rb = pair(s[mt][n], 1);
 #pragma unroll
                     for (int p = 0; p < X::NP; ++p) {
-                        const uint32_t wa = pack2(r0, r1, C), wb = pack2(r2, r3, C);
+                        const uint32_t wa = pack2(ra.x, ra.y, C), wb = pack2(rb.x, rb.y, C);
                         pp[mt][n][p][0] = transpose8x8(wa);
                         pp[mt][n][p][1] = transpose8x8(wb);
-                        const float2 fa = unpack2(wa, C), fb = unpack2(wb, C);
-                        r0 -= fa.x, r1 -= fa.y, r2 -= fb.x, r3 -= fb.y;
+                        ra = sub2(ra, unpack2(wa, C)), rb = sub2(rb, unpack2(wb, C));
+                        if constexpr (X::f16) ra = mul2(ra, make_float2(kRest, kRest)), rb = mul2(rb, make_float2(kRest, kRest));
                     }
                 }
             const uint32_t v_addr = v_base + ((lane & 7) + (lane >> 4) * 8) * X::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-                float acc[NT][4];
+                float acc[NT][4], rest[NT][4];  // rest: of f16's second parts
 #pragma unroll
-                for (int n = 0; n < NT; ++n) begin(acc[n], o[i][n]);
+                for (int n = 0; n < NT; ++n) {
+                    begin(acc[n], o[i][n]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) rest[n][e] = 0.f;
+                }
 #pragma unroll
                 for (int mt = 0; mt < X::MT; ++mt) {
                     uint32_t w[4];
@@ -829,10 +839,17 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int p = X::NP - 1; p >= 0; --p) mma16<X::bf>(acc[n], w, pp[mt][n][p][0], pp[mt][n][p][1]);
+                        for (int p = X::NP - 1; p >= 0; --p)
+                            mma16<X::bf>(X::f16 && p == 1 ? rest[n] : acc[n], w, pp[mt][n][p][0], pp[mt][n][p][1]);
                 }
 #pragma unroll
-                for (int n = 0; n < NT; ++n) finish(o[i][n], acc[n]);
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (X::f16)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            set_pair(acc[n], e, fma2(pair(rest[n], e), make_float2(1.f / kRest, 1.f / kRest), pair(acc[n], e)));
+                    finish(o[i][n], acc[n]);
+                }
             }
         }
     }

@@ -1,9 +1,9 @@
 """What the paged cache operators promise, where it is easiest to break: quotients at the edge
-of a half step.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
+of a half step, weights far below a row's largest.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
 import numpy as np
 import pytest
 
-from test_paged_gpu import cache, q8_blocks
+from test_paged_gpu import attention_ref, cache, check_attention, dtype, q8_blocks
 
 pytestmark = pytest.mark.gpu
 
@@ -47,4 +47,43 @@ def test_q8_quotients_next_to_every_half(cuda, tirlib, orc, entry):
         quants, d = q8_blocks(orc, y)
         assert torch.equal(pool[at], torch.from_numpy(quants).cuda())
         assert torch.equal(steps[at], torch.from_numpy(d).cuda())
+    tirlib.ops_check()
+
+
+def write_rows(torch, tirlib, kv, k, v):
+    """k, v [positions, kv_heads, dim] f32 into row 0 of the cache."""
+    pos = torch.arange(k.shape[0], dtype=torch.int32, device="cuda")
+    tirlib.kv_append(kv, k.contiguous(), v.contiguous(), torch.zeros_like(pos), pos)
+
+
+FAR = [("f32", "f32"), ("f32", "bf16"), ("f32", "f16"), ("f16", "f16"), ("bf16", "bf16")]
+
+
+@pytest.mark.parametrize("lead", [12.0, 16.0, 21.0, 25.0])
+@pytest.mark.parametrize("where", [100, 15000])
+@pytest.mark.parametrize("act,kind", FAR)
+def test_weights_far_below_a_leading_key(cuda, tirlib, act, kind, where, lead):
+    """One key leads a long row by many natural units; its value is zero, so the output is
+    what the small weights make of the others' values, all of one sign.  Undivided
+    (max_len 1) and divided."""
+    torch = cuda
+    n, dim = 20000, 64
+    g = torch.Generator("cuda").manual_seed(int(lead) + where)
+    kv, values, _ = cache(torch, tirlib, kind, 1, n, 1, dim, 16, seed=3)
+    k = 0.1 * torch.randn(n, 1, dim, device="cuda", generator=g)
+    k[:, 0, 0] = 0.0
+    k[where] = 0.0
+    k[where, 0, 0] = 8.0
+    v = 1024 * (0.5 + torch.rand(n, 1, dim, device="cuda", generator=g))  # f16 outputs stay above its smallest normal value
+    v[where] = 0.0
+    write_rows(torch, tirlib, kv, k, v)
+    q = torch.randn(1, 4, dim, device="cuda", generator=g)
+    q[..., 0] = lead / 8.0 / 0.125
+    q = q.to(dtype(torch, act))
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    ref = attention_ref(torch, q, values(), [n], 0.125, 0)
+    for max_len in (1, n):
+        out = torch.empty_like(q)
+        tirlib.paged_attention(q, kv, lens, out, max_len=max_len)
+        check_attention(torch, out, *ref, dim, n)
     tirlib.ops_check()
