@@ -272,10 +272,16 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     constexpr uint32_t FULL = 0xffffffffu;
     constexpr int CH = X::ROW / 16;        // 16-byte pieces of a cached row
     constexpr int LPR = CH < 8 ? CH : 8;  // lanes that copy a row
-    // weights are 2^kLift above their logarithm's reference, which may lag the maximum by
-    // kLag: weights in f16 parts fill its range from the top (2^15)
-    constexpr float kLift = X::f16 ? 11.f : X::q8 ? 6.f : 0.f;
-    constexpr float kLag = X::f16 ? 4.f : 8.f;
+    // Weights are 2^kLift above their logarithm's reference, which may lag the maximum by
+    // kLag: those in f16 parts fill its range from the top (2^15).  Their second part is
+    // kept kRest above its place, in a sum of its own: in its place its digits would end
+    // with f16's range, from weights of 2^-12 of the reference's on (a key that leads the
+    // row by 8), and a long row sums 10^5 of those.  So 20 bits remain down to 2^-28 (19),
+    // 12 to 2^-36 (25); in Q8_0 of weights times steps, beside the largest step.
+    constexpr bool kSmall = X::f16 || X::q8;
+    constexpr float kLift = kSmall ? 11.f : 0.f;
+    constexpr float kLag = kSmall ? 4.f : 8.f;
+    constexpr float kRest = 4096.f;
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* ring = smem;
     uint32_t* qf = reinterpret_cast<uint32_t*>(smem + X::RING);
@@ -718,16 +724,24 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 #pragma unroll
             for (int e = 0; e < 2; ++e) set_pair(sum, e, F32Q ? add2(pair(sum, e), pair(acc, e)) : pair(acc, e));
         };
+        auto add_rest = [&](float* acc, const float* rest) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) set_pair(acc, e, fma2(pair(rest, e), make_float2(1.f / kRest, 1.f / kRest), pair(acc, e)));
+        };
         if constexpr (X::q8) {
             const float inv = __uint_as_float(static_cast<uint32_t>(127 + 14 - v_exp) << 23);
             const uint32_t v_addr = v_base + (lane & 15) * X::PITCH + (lane >> 4) * 16;
 #pragma unroll
             for (int b = 0; b < D / 32; ++b) {
-                float acc[2][NT][4];
+                float acc[2][NT][4], rest[2][NT][4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) begin(acc[i][n], o[2 * b + i][n]);
+                    for (int n = 0; n < NT; ++n) {
+                        begin(acc[i][n], o[2 * b + i][n]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) rest[i][n][e] = 0.f;
+                    }
 #pragma unroll
                 for (int mt = 0; mt < X::MT; ++mt) {
                     const float d0 = v_steps[mt][0].get(b) * inv, d1 = v_steps[mt][1].get(b) * inv;
@@ -736,7 +750,8 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                     for (int n = 0; n < NT; ++n) {
                         const float2 wa = mul2(pair(s[mt][n], 0), make_float2(d0, d0)), wb = mul2(pair(s[mt][n], 1), make_float2(d1, d1));
                         const __half2 ha = __float22half2_rn(wa), hb = __float22half2_rn(wb);
-                        const float2 ra = sub2(wa, __half22float2(ha)), rb = sub2(wb, __half22float2(hb));
+                        const float2 up = make_float2(kRest, kRest);
+                        const float2 ra = mul2(sub2(wa, __half22float2(ha)), up), rb = mul2(sub2(wb, __half22float2(hb)), up);
                         p0[n][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&ha));
                         p0[n][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hb));
                         p1[n][0] = transpose8x8(pack2(ra.x, ra.y, Elem::F16));
@@ -749,7 +764,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                         q8_pairs(w[2 * i], &x[i][0], &x[i][1]);
                         q8_pairs(w[2 * i + 1], &x[i][2], &x[i][3]);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma16<false>(acc[i][n], x[i], p1[n][0], p1[n][1]);
+                        for (int n = 0; n < NT; ++n) mma16<false>(rest[i][n], x[i], p1[n][0], p1[n][1]);
                     }
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
@@ -759,7 +774,10 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) finish(o[2 * b + i][n], acc[i][n]);
+                    for (int n = 0; n < NT; ++n) {
+                        add_rest(acc[i][n], rest[i][n]);
+                        finish(o[2 * b + i][n], acc[i][n]);
+                    }
             }
         } else if constexpr (X::tf32) {
             uint32_t ph[X::MT][2][NT][2], pl[X::MT][2][NT][2];
@@ -802,11 +820,6 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                 for (int n = 0; n < NT; ++n) finish(o[i][n], acc[n]);
             }
         } else {
-            // f16's second part of a weight is kept 2^12 above its place, in a sum of its own:
-            // in its place its digits would end with f16's range, from weights of 2^-12 of the
-            // reference's on (a key that leads the row by 8), and a long row sums 10^5 of those.
-            // So 20 bits remain down to 2^-28 (19), 12 to 2^-36 (25).
-            constexpr float kRest = 4096.f;
             uint32_t pp[X::MT][NT][X::NP][2];
 #pragma unroll
             for (int mt = 0; mt < X::MT; ++mt)
@@ -819,13 +832,13 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                         pp[mt][n][p][0] = transpose8x8(wa);
                         pp[mt][n][p][1] = transpose8x8(wb);
                         ra = sub2(ra, unpack2(wa, C)), rb = sub2(rb, unpack2(wb, C));
-                        if constexpr (X::f16) ra = mul2(ra, make_float2(kRest, kRest)), rb = mul2(rb, make_float2(kRest, kRest));
+                        if constexpr (kSmall) ra = mul2(ra, make_float2(kRest, kRest)), rb = mul2(rb, make_float2(kRest, kRest));
                     }
                 }
             const uint32_t v_addr = v_base + ((lane & 7) + (lane >> 4) * 8) * X::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-                float acc[NT][4], rest[NT][4];  // rest: of f16's second parts
+                float acc[NT][4], rest[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     begin(acc[n], o[i][n]);
@@ -840,14 +853,11 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int p = X::NP - 1; p >= 0; --p)
-                            mma16<X::bf>(X::f16 && p == 1 ? rest[n] : acc[n], w, pp[mt][n][p][0], pp[mt][n][p][1]);
+                            mma16<X::bf>(kSmall && p == 1 ? rest[n] : acc[n], w, pp[mt][n][p][0], pp[mt][n][p][1]);
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    if constexpr (X::f16)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            set_pair(acc[n], e, fma2(pair(rest[n], e), make_float2(1.f / kRest, 1.f / kRest), pair(acc[n], e)));
+                    if constexpr (kSmall) add_rest(acc[n], rest[n]);
                     finish(o[i][n], acc[n]);
                 }
             }

@@ -56,7 +56,7 @@ def write_rows(torch, tirlib, kv, k, v):
     tirlib.kv_append(kv, k.contiguous(), v.contiguous(), torch.zeros_like(pos), pos)
 
 
-FAR = [("f32", "f32"), ("f32", "bf16"), ("f32", "f16"), ("f16", "f16"), ("bf16", "bf16")]
+FAR = [("f32", "f32"), ("f32", "bf16"), ("f32", "f16"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "q8_0"), ("f16", "q8_0"), ("bf16", "q8_0")]
 
 
 @pytest.mark.parametrize("lead", [12.0, 16.0, 21.0, 25.0])
@@ -86,4 +86,40 @@ def test_weights_far_below_a_leading_key(cuda, tirlib, act, kind, where, lead):
         out = torch.empty_like(q)
         tirlib.paged_attention(q, kv, lens, out, max_len=max_len)
         check_attention(torch, out, *ref, dim, n)
+    tirlib.ops_check()
+
+
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("differ", ["blocks", "positions"])
+def test_q8_values_of_very_different_steps(cuda, tirlib, act, differ):
+    """Q8_0 values whose steps differ by up to 2^24: between the blocks of a head, and between
+    positions of which those of large steps have next to no weight.  Every element against
+    its own values' size."""
+    torch = cuda
+    n, dim = 700, 64
+    g = torch.Generator("cuda").manual_seed(5)
+    kv, values, _ = cache(torch, tirlib, "q8_0", 1, n, 2, dim, 16, seed=4)
+    q = torch.randn(1, 8, dim, device="cuda", generator=g)
+    kv.v_scale.copy_(torch.exp2(-14.0 + torch.rand(kv.v_scale.shape, device="cuda", generator=g)))
+    if differ == "blocks":
+        kv.v_scale[..., 0] *= 2.0 ** 22
+    else:
+        big = kv.table[0, ::5].long()
+        kv.v_scale[big] *= 2.0 ** 22
+        q[..., 0] = 40.0
+        kv.k[..., 0] = 40
+        kv.k[big, ..., 0] = -120
+        kv.k_scale[..., 0] = 2.0 ** -5
+    q = q.to(dtype(torch, act))
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    ref, mass, big_score = attention_ref(torch, q, values(), [n], 0.125, 0)
+    for max_len in (1, n):
+        out = torch.empty_like(q)
+        tirlib.paged_attention(q, kv, lens, out, max_len=max_len)
+        tiny = 2.0 ** -25 if act == "f16" else 0.0  # half a step of f16 below its normal range
+        ut = torch.finfo(dtype(torch, act)).eps / 2
+        e = (2 * dim / 8 + 4) * 2.0 ** -23 * big_score + 2.0 ** -20
+        bound = (2 * e + n / 8 * 2.0 ** -23 + 2.0 ** -20) * mass + ut * ref.abs() + tiny
+        err = (out.double() - ref).abs()
+        assert (err <= bound).all(), float((err / bound).max())
     tirlib.ops_check()
