@@ -23,8 +23,8 @@
 // blocks into the operand layout of P'.
 //
 // Operand types.  K and V enter as they are stored: f16 / bf16 directly, Q8_0
-// quants as exact f16 values (the values' n, the keys' (128 + n) 2^-24) with the
-// block steps applied outside, f32 split into two tf32 parts.  q and the weights p are split into as many parts as they
+// quants as exact f16 integers with the block steps applied outside, f32 split
+// into two tf32 parts.  q and the weights p are split into as many parts as they
 // need: 16-bit queries are exact in one (bf16 ones scaled by a power of two for
 // f16), f32 queries take two f16 (22 bits under a per-head power of two), three
 // bf16 or two tf32 parts.  p has two bf16 parts (16 bits, below the rounding of a
@@ -137,14 +137,6 @@ __device__ __forceinline__ void mma16(float* d, const uint32_t* a, uint32_t b0, 
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// d = c + a b, f16 operands
-__device__ __forceinline__ void mma16_from(float* d, const float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
-}
-
 // d (16 x 8, f32) += a (16 x 8) b (8 x 8), tf32 operands
 __device__ __forceinline__ void mma8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm(
@@ -172,22 +164,16 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // Four int8 as exact f16 integers: bytes 0 and 2 in *even, 1 and 3 in *odd.  The
-// byte 128 + n under the exponent of 1024 reads 1152 + n.
+// byte 128 + n under the exponent of 1024 reads 1152 + n.  (Leaving the 128 in, as f16's
+// denormals (128 + n) 2^-24, and taking 128 sum q off the keys' products spares two of five
+// operations, but such a sum has f32's steps at 128 sum q: with quants below 4 beside one of
+// 127 outputs were off by 3e-5, without the 128 by 3e-7.)
 __device__ __forceinline__ void q8_pairs(uint32_t w, uint32_t* even, uint32_t* odd) {
     const uint32_t a = (w & 0x00ff00ffu) ^ 0x64806480u, b = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
     const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
     const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
     *even = *reinterpret_cast<const uint32_t*>(&x);
     *odd = *reinterpret_cast<const uint32_t*>(&y);
-}
-
-// The same as (128 + n) 2^-24, f16's denormals: three operations instead of five
-// where the 128 can be taken off the sum (the keys: by what an accumulator starts
-// from; it is of the sum's own size there, so nothing is lost to it.  The values'
-// sums run over the positions, where it would outgrow them).
-__device__ __forceinline__ void q8_pairs_biased(uint32_t w, uint32_t* even, uint32_t* odd) {
-    *even = (w & 0x00ff00ffu) ^ 0x00800080u;
-    *odd = ((w >> 8) & 0x00ff00ffu) ^ 0x00800080u;
 }
 
 // The Q8_0 steps of one position's head: D / 32 halves in one load.
@@ -246,8 +232,7 @@ struct AttnCfg {
     static constexpr int WARPS = HALF > 16 * 1024 && NT == 2 ? 2 : 4;  // two where q takes the room
     static constexpr int THREADS = WARPS * 32;
     static constexpr int UNIT = WARPS * TILE;
-    static constexpr int BIAS = q8 ? HEADS * (D / 32) * 4 : 0;
-    static constexpr int FIXED = QBYTES + HEADS * 4 + WARPS * HEADS * 8 + BIAS;
+    static constexpr int FIXED = QBYTES + HEADS * 4 + WARPS * HEADS * 8;
     // a warp's ring: SLOTS half tiles (keys, values, keys, ...), an odd number, so that
     // a step on keys asks for keys.  Three CTAs an SM for heads of 64 (64 x 256 in f32:
     // 12.5 us, 13.2 with two), two for wider ones where three slots fit (64 x 2048 in
@@ -287,7 +272,6 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
     uint32_t* qf = reinterpret_cast<uint32_t*>(smem + X::RING);
     float* cs = reinterpret_cast<float*>(smem + X::RING + X::QBYTES);
     float* ml = cs + X::HEADS;  // [WARPS][HEADS][2]
-    float* bias = ml + X::WARPS * X::HEADS * 2;  // Q8_0: [D / 32][HEADS]
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int tiles = kv.kv_heads * a.head_tiles;
@@ -428,7 +412,6 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                 for (int i = 0; i < D / 32; ++i) x[i] *= up;
             }
         }
-        if constexpr (X::q8) c *= 16777216.f;  // the keys' 2^-24
         if (lane == 0) cs[j] = fmaxf(c, 1.2e-38f);  // never 0: a masked score is c * -inf
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -455,12 +438,6 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                         *p = __half_as_ushort(b);
                         rem -= __half2float(b);
                     }
-                }
-                if constexpr (X::q8) {
-                    float sum = x[i] - rem;  // what the parts hold
-#pragma unroll
-                    for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(FULL, sum, w);
-                    if (lane == 0) bias[i * X::HEADS + j] = -128.f / 16777216.f * sum;
                 }
             }
         }
@@ -496,15 +473,6 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
-    float off[X::q8 ? D / 32 : 1][NT][2];
-    if constexpr (X::q8) {
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) off[b][n][e] = bias[b * X::HEADS + n * 8 + 2 * t + e];
-    }
     int v_exp = 0;  // Q8_0: o is kept over 2^(v_exp - 14), the power of two above the steps seen so far
 
     // c s - base.  The product is rounded (or exact: c is a power of two under f32
@@ -560,19 +528,19 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
                 for (int b = 0; b < D / 32; ++b) {
                     uint32_t w[4], x0[4], x1[4];
                     ldsm4(w, k_addr + b * 32);
-                    q8_pairs_biased(w[0], &x0[0], &x0[2]);
-                    q8_pairs_biased(w[1], &x0[1], &x0[3]);
-                    q8_pairs_biased(w[2], &x1[0], &x1[2]);
-                    q8_pairs_biased(w[3], &x1[1], &x1[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t* x = i < 2 ? x0 : x1;
+                        q8_pairs(w[i], &x[i & 1], &x[2 + (i & 1)]);
+                    }
                     const float d0 = k_steps[0].get(b), d1 = k_steps[1].get(b);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const float from[4] = {off[b][n][0], off[b][n][1], off[b][n][0], off[b][n][1]};
-                        float sum[4];
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int p = X::NQ - 1; p >= 0; --p) {
                             const uint2 q0 = q_op(2 * b, n, p), q1 = q_op(2 * b + 1, n, p);
-                            mma16_from(sum, p == X::NQ - 1 ? from : sum, x0, q0.x, q0.y);
+                            mma16<false>(sum, x0, q0.x, q0.y);
                             mma16<false>(sum, x1, q1.x, q1.y);
                         }
                         s[mt][n][0] = fmaf(sum[0], d0, s[mt][n][0]);

@@ -1,5 +1,7 @@
 """What the paged cache operators promise, where it is easiest to break: quotients at the edge
 of a half step, weights far below a row's largest.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
+import math
+
 import numpy as np
 import pytest
 
@@ -123,3 +125,23 @@ def test_q8_values_of_very_different_steps(cuda, tirlib, act, differ):
         err = (out.double() - ref).abs()
         assert (err <= bound).all(), float((err / bound).max())
     tirlib.ops_check()
+
+
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_q8_keys_with_one_large_channel(cuda, tirlib, act, dim):
+    """Every block of keys has one channel far above the others, which sets its step, and the
+    query looks away from it: the small quants carry the scores."""
+    torch = cuda
+    n = 500
+    g = torch.Generator("cuda").manual_seed(6)
+    kv, values, _ = cache(torch, tirlib, "q8_0", 1, n, 1, dim, 16, seed=7)
+    kv.k.copy_(torch.randint(-3, 4, kv.k.shape, device="cuda", generator=g, dtype=torch.int8))
+    kv.k[..., ::32] = 127
+    kv.k_scale.fill_(1.0)
+    q = (0.5 + torch.rand(1, 8, dim, device="cuda", generator=g)).to(dtype(torch, act))
+    q[..., ::32] = 0
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    tirlib.paged_attention(q, kv, lens, out)
+    check_attention(torch, out, *attention_ref(torch, q, values(), [n], 1 / math.sqrt(dim), 0), dim, n)
