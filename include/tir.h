@@ -411,7 +411,9 @@ tir_status tir_attention(const float *q, const float *k_cache, const float *v_ca
  * `stream` of the current device and can be captured into a graph after one
  * earlier call on that device.  They allocate nothing.  What the host cannot
  * check (a page id outside the pool, a position outside the table) is skipped
- * by the kernels and reported by tir_ops_check as TIR_ERR_INVALID_ARG. */
+ * by the kernels and reported by tir_ops_check as TIR_ERR_INVALID_ARG: nothing
+ * is written or read there, and in attention the positions of such a page have
+ * no part in the softmax (a row that has no others gets zeros). */
 
 /* Element types beside TIR_DTYPE_F32 and TIR_DTYPE_Q8_0 (GGUF's codes). */
 enum { TIR_DTYPE_F16 = 1, TIR_DTYPE_BF16 = 30 };

@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join(const AttnArg
 #pragma unroll 4
     for (int i = warp; i < range.used; i += kJoinWarps) {
         const float2 x = *reinterpret_cast<const float2*>(ml + 2 * i);
-        const float f = x.x == -INFINITY ? 0.f : exp2_fast(x.x - top);
+        const float f = part_factor(x.x, top);
         l = fmaf(f, x.y, l);
 #pragma unroll
         for (int e = 0; e < N; e += 2) {
@@ -58,6 +58,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join(const AttnArg
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) sum += sums[w];
+    sum = part_sum(sum, top);
     for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
         float y = 0.f;
 #pragma unroll

@@ -163,6 +163,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// Parts (m, l, o) of a row count 2^(m - top) times.  One without a position on a page of the
+// pool has m = -inf, and a row of such parts gets zeros; one whose scores are all -inf has
+// kNoWeight, below every other, and a row of such parts 0 / 0.
+constexpr float kNoWeight = -3.402823466e38f;
+__device__ __forceinline__ float part_factor(float m, float top) { return m == -INFINITY ? 0.f : exp2_fast(m - top); }
+__device__ __forceinline__ float part_sum(float sum, float top) { return top == -INFINITY ? 1.f : sum; }
+
 // Four int8 as exact f16 integers: bytes 0 and 2 in *even, 1 and 3 in *odd.  The
 // byte 128 + n under the exponent of 1024 reads 1152 + n.  (Leaving the 128 in, as f16's
 // denormals (128 + n) 2^-24, and taking 128 sum q off the keys' products spares two of five
@@ -337,7 +344,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         return pos < range.k1 ? page_id(kv, row, pos) : -1;
     };
     // where this lane's position of tile i lies, in 16-byte units; kNowhere past the
-    // end or on a bad page: zeros instead
+    // end or on a bad page: zeros are copied instead, and its score is -inf
     constexpr uint32_t kNowhere = 0xffffffffu;
     const uint32_t head_at = hk * kv.head16;
     auto place = [&](int i, int32_t page) -> uint32_t {
@@ -377,15 +384,17 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 #pragma unroll
         for (int i = 0; i <= X::AHEAD; ++i) pages[i] = lookup(i);
     }
+    uint32_t live[X::AHEAD];  // of the tiles asked for, in order: bit p (TILE 16: p + 16, too) for position p
 #pragma unroll
     for (int i = 0; i < X::AHEAD; ++i) {
         const uint32_t at = place(i, pages[i]);
-        const bool full = __all_sync(FULL, at != kNowhere);
-        if (i < my_tiles) issue(2 * i, at, full, kv.k, kv.ks);
+        live[i] = __ballot_sync(FULL, at != kNowhere);
+        if (i < my_tiles) issue(2 * i, at, live[i] == FULL, kv.k, kv.ks);
         cp_async_commit();
-        if (i < my_tiles) issue(2 * i + 1, at, full, kv.v, kv.vs);
+        if (i < my_tiles) issue(2 * i + 1, at, live[i] == FULL, kv.v, kv.vs);
         cp_async_commit();
     }
+    uint32_t any_live = 0u;
     int32_t next_page = pages[X::AHEAD];
 
     // ---- q operands, while the first tiles are on their way ----
@@ -496,7 +505,12 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         __syncwarp();
         const bool more = it + X::AHEAD < my_tiles;
         const uint32_t ahead = place(it + X::AHEAD, next_page);
-        const bool full = __all_sync(FULL, ahead != kNowhere);
+        const uint32_t now = live[0];
+        any_live |= now;
+#pragma unroll
+        for (int i = 0; i + 1 < X::AHEAD; ++i) live[i] = live[i + 1];
+        live[X::AHEAD - 1] = __ballot_sync(FULL, ahead != kNowhere);
+        const bool full = live[X::AHEAD - 1] == FULL;
         if (more) issue(free_slot, ahead, full, kv.k, kv.ks);
         cp_async_commit();
         next_page = lookup(it + X::AHEAD + 1);
@@ -594,15 +608,14 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 
         // weights: p = 2^(t - m + lift), with m moved only when a score passes it by
         // more than kLag (rare after the first tiles): no reduction in the usual tile
-        const int32_t left = range.k1 - (range.k0 + (it * X::WARPS + warp) * X::TILE);  // positions of this tile
-        if (left < X::TILE) {
+        if (now != FULL) {
 #pragma unroll
             for (int mt = 0; mt < X::MT; ++mt)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (mt * 16 + g + (e >> 1) * 8 >= left) s[mt][n][e] = -INFINITY;
+                        if (!(now >> (mt * 16 + g + (e >> 1) * 8) & 1u)) s[mt][n][e] = -INFINITY;
         }
         bool moves = false;
         float top[NT][2];
@@ -854,7 +867,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(FULL, l[n][e], w);
             if (g == 0) {
-                ml[(warp * X::HEADS + j) * 2] = m[n][e];
+                ml[(warp * X::HEADS + j) * 2] = any_live ? fmaxf(m[n][e], kNoWeight) : m[n][e];
                 ml[(warp * X::HEADS + j) * 2 + 1] = l[n][e];
             }
 #pragma unroll
@@ -876,8 +889,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
         for (int w = 0; w < X::WARPS; ++w) top = fmaxf(top, ml[(w * X::HEADS + j) * 2]);
 #pragma unroll
         for (int w = 0; w < X::WARPS; ++w) {
-            const float mw = ml[(w * X::HEADS + j) * 2];
-            const float f = mw == -INFINITY ? 0.f : exp2_fast(mw - top);
+            const float f = part_factor(ml[(w * X::HEADS + j) * 2], top);
             const float lw = ml[(w * X::HEADS + j) * 2 + 1];
             sum += f * lw;
             const float* part = reinterpret_cast<const float*>(ring + w * X::SLOTS * X::HALF) + j * (D + 4) + d;
@@ -885,6 +897,7 @@ __global__ void __launch_bounds__(AttnCfg<C, D, NT, F32Q>::THREADS, AttnCfg<C, D
             for (int e = 0; e < 8; ++e) y[e] = fmaf(f, part[e], y[e]);
         }
         if (range.used == 1) {
+            sum = part_sum(sum, top);
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = y[e] / sum;
             const int64_t at = row * a.out_stride + static_cast<int64_t>(h0 + j) * D + d;

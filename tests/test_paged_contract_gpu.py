@@ -1,5 +1,5 @@
 """What the paged cache operators promise, where it is easiest to break: quotients at the edge
-of a half step, weights far below a row's largest.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
+of a half step, weights far below a row's largest, pages outside the pool.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
 import math
 
 import numpy as np
@@ -145,3 +145,51 @@ def test_q8_keys_with_one_large_channel(cuda, tirlib, act, dim):
     out = torch.empty_like(q)
     tirlib.paged_attention(q, kv, lens, out)
     check_attention(torch, out, *attention_ref(torch, q, values(), [n], 1 / math.sqrt(dim), 0), dim, n)
+
+
+def attention_over(torch, q, vals, seen, scale):
+    """float64 outputs of row 0 over the positions of the mask `seen`; zeros for none."""
+    rows, qh, dim = q.shape
+    out = torch.zeros(rows, qh, dim, dtype=torch.float64, device="cuda")
+    mass, big = torch.zeros_like(out), torch.zeros(rows, qh, 1, dtype=torch.float64, device="cuda")
+    for r in range(rows):
+        if not seen[r].any():
+            continue
+        K, V = vals[r, :, 0][seen[r]], vals[r, :, 1][seen[r]]
+        for h in range(qh):
+            kh = h // (qh // K.shape[1])
+            x = (K[:, kh] @ q[r, h].double()) * scale
+            p = torch.softmax(x, 0)
+            out[r, h], mass[r, h] = p @ V[:, kh], p @ V[:, kh].abs()
+            big[r, h] = (K[:, kh].abs() @ q[r, h].double().abs()).max() * scale
+    return out, mass, big
+
+
+@pytest.mark.parametrize("act,kind", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "q8_0")])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_positions_on_a_bad_page_take_no_part(cuda, tirlib, act, kind, dim):
+    """Pages outside the pool, at the start, inside and at the end of a row, and a row of
+    nothing else: the softmax is over the other positions, and zeros where there are none."""
+    torch = cuda
+    n, page, rows = 2100, 7, 4
+    kv, values, _ = cache(torch, tirlib, kind, rows, n, 1, dim, page, seed=8)
+    vals = values()
+    seen = torch.ones(rows, vals.shape[1], dtype=torch.bool, device="cuda")
+    seen[:, n:] = False
+    bad = {0: [0, 1, 5, 40, 41, 42, 43, 44, 45, 200, 299], 1: list(range(kv.table.shape[1])), 2: list(range(1, kv.table.shape[1]))}
+    for r, pages in bad.items():
+        for i, p in enumerate(pages):
+            kv.table[r, p] = (-1, 1 << 30, -(1 << 31), kv.k.shape[0])[i % 4]
+            seen[r, p * page:(p + 1) * page] = False
+    q = torch.randn(rows, 4, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(9)).to(dtype(torch, act))
+    lens = torch.full((rows,), n, dtype=torch.int32, device="cuda")
+    ref = attention_over(torch, q, vals, seen, 1 / math.sqrt(dim))
+    for max_len in (1, n):
+        out = torch.full_like(q, 3.0)
+        tirlib.paged_attention(q, kv, lens, out, max_len=max_len)
+        check_attention(torch, out, *ref, dim, n)
+        assert (out[1] == 0).all()
+        with pytest.raises(tirlib.TirError) as e:
+            tirlib.ops_check()
+        assert e.value.name == "INVALID_ARG" and "page id" in e.value.message
+    tirlib.ops_check()
