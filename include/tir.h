@@ -496,8 +496,11 @@ tir_status tir_kv_gather(const tir_kv_pages *kv, void *k_out, int64_t k_out_stri
  * row of length 0 gets zeros.  scale multiplies the scores (0: 1 / sqrt(dim)).
  * out has q's type.  f32 queries go with any cache, 16-bit ones with a cache of
  * their own type or Q8_0.  What lies outside a row's positions is never used,
- * whatever it holds; a NaN or infinity inside makes the head's output
- * non-finite.  Several query tokens of one sequence are rows of their own, with
+ * whatever it holds.  Inside, a NaN in a key or a score of +inf makes the head's
+ * output non-finite, a NaN or infinity in a value its element of the output
+ * (Q8_0: its block of 32); a key with an infinity whose score is -inf has no
+ * weight, as in the formula, or makes the head non-finite, and a row of nothing
+ * else is non-finite.  Several query tokens of one sequence are rows of their own, with
  * the same pages in the table and lengths that end at each.  max_len, at least
  * the longest length (0: what the table holds), only sizes the split of long
  * rows over the GPU.  workspace: tir_paged_attention_workspace bytes (0: none

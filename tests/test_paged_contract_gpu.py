@@ -1,5 +1,6 @@
 """What the paged cache operators promise, where it is easiest to break: quotients at the edge
-of a half step, weights far below a row's largest, pages outside the pool.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
+of a half step, weights far below a row's largest, pages outside the pool, infinities inside
+a row.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
 import math
 
 import numpy as np
@@ -192,4 +193,56 @@ def test_positions_on_a_bad_page_take_no_part(cuda, tirlib, act, kind, dim):
         with pytest.raises(tirlib.TirError) as e:
             tirlib.ops_check()
         assert e.value.name == "INVALID_ARG" and "page id" in e.value.message
+    tirlib.ops_check()
+
+
+@pytest.mark.parametrize("act,kind", FAR)
+@pytest.mark.parametrize("max_len", [1, 0])
+def test_nan_and_infinity_inside_a_row(cuda, tirlib, act, kind, max_len):
+    """A NaN in a key, or a NaN or infinity in a value, makes the heads that read it
+    non-finite; a key of score -inf has no weight or makes its head non-finite, one of
+    +inf makes it non-finite; the other row and the other key-value head are as they were."""
+    torch = cuda
+    n, dim, inf = 3000, 64, float("inf")
+    kv, values, _ = cache(torch, tirlib, kind, 2, n, 2, dim, 16, seed=11)
+    q = torch.randn(2, 4, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(12))
+    q[..., 5] = 1.0 + q[..., 5].abs()
+    q = q.to(dtype(torch, act))
+    lens = torch.tensor([n, n], dtype=torch.int32, device="cuda")
+    clean = torch.empty_like(q)
+    tirlib.paged_attention(q, kv, lens, clean, max_len=max_len)
+    pos = 1234
+    page, slot = int(kv.table[0, pos // 16]), pos % 16
+    q8 = kind == "q8_0"
+    pools = (kv.k_scale, kv.v_scale) if q8 else (kv.k, kv.v)
+    for what, x in (("k", float("nan")), ("k", inf), ("k", -inf), ("v", float("nan")), ("v", inf), ("v", -inf)):
+        pool = pools[what == "v"]
+        c = 0 if q8 else 5
+        old = pool[page, slot, 0, c].clone()
+        pool[page, slot, 0, c] = x
+        score = 0.0
+        if what == "k" and x == x:  # sign of the score
+            score = x if not q8 else None
+        out = torch.empty_like(q)
+        tirlib.paged_attention(q, kv, lens, out, max_len=max_len)
+        assert torch.equal(out[1], clean[1]) and torch.equal(out[0, 2:], clean[0, 2:]), (what, x)
+        if what == "v":
+            d = slice(0, 32) if q8 else 5
+            assert not torch.isfinite(out[0, :2, d]).any(), (what, x)
+        elif x != x or score == inf:
+            assert not torch.isfinite(out[0, :2]).any(), (what, x)
+        else:
+            pool[page, slot, 0, c] = old
+            seen = torch.ones(2, values().shape[1], dtype=torch.bool, device="cuda")
+            seen[:, n:] = False
+            seen[0, pos] = False
+            ref = attention_over(torch, q, values(), seen, 0.125)
+            for h in range(2):
+                if torch.isfinite(out[0, h]).all():
+                    check_attention(torch, out[:1, h:h + 1], *(y[:1, h:h + 1] for y in ref), dim, n)
+        pool[page, slot, 0, c] = old
+    pools[0][kv.table[0].long(), :, 0, 0 if q8 else 5] = -inf
+    out = torch.empty_like(q)
+    tirlib.paged_attention(q, kv, lens, out, max_len=max_len)
+    assert not torch.isfinite(out[0, :2]).any() and torch.equal(out[1], clean[1]) and torch.equal(out[0, 2:], clean[0, 2:])
     tirlib.ops_check()
