@@ -1345,7 +1345,7 @@ tir_status tir_ops_check(void* stream) {
         return fail(TIR_ERR_TIMEOUT, "a device-side wait of an op launched on device " + std::to_string(dev) +
                                          " gave up (TIR_TIMEOUT_MS); its outputs are incomplete");
     uint32_t bad = 0;
-    const tir_status prc = paged_take_error(dev, &bad);
+    const tir_status prc = paged_take_error(dev, stream, &bad);
     if (prc != TIR_OK) return prc;
     if (bad != 0u)
         return fail(TIR_ERR_INVALID_ARG, "a paged cache operator on device " + std::to_string(dev) + " met" +

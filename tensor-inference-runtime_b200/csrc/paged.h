@@ -45,8 +45,9 @@ tir_status check_rows(const void* p, int64_t stride, int64_t heads, int64_t dim,
                       const char* what);
 // The error word of the current device (looked up on its first use there).
 tir_status paged_error_word(uint32_t** out);
-// Reads and clears `device`'s error word; 0 where no paged operator ran on it.
-tir_status paged_take_error(int device, uint32_t* bits);
+// Takes the error word of `device`, the current one, on `stream` and waits; 0 where no
+// paged operator ran on it.
+tir_status paged_take_error(int device, void* stream, uint32_t* bits);
 tir_status paged_fail(cudaError_t e, const char* what);
 
 }  // namespace tir

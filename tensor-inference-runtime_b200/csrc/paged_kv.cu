@@ -24,8 +24,12 @@
 namespace tir {
 
 static __device__ uint32_t g_paged_err;
+static __device__ uint32_t g_paged_taken;
 
 namespace {
+
+// One step: a bit that another stream sets meanwhile is either taken or stays.
+__global__ void take_error_kernel() { g_paged_taken = atomicExch(&g_paged_err, 0u); }
 
 constexpr uint32_t FULL = 0xffffffffu;
 constexpr int kRowThreads = 128;
@@ -606,16 +610,15 @@ tir_status paged_error_word(uint32_t** out) {
     return TIR_OK;
 }
 
-tir_status paged_take_error(int device, uint32_t* bits) {
+tir_status paged_take_error(int device, void* stream, uint32_t* bits) {
     *bits = 0u;
-    uint32_t* p = nullptr;
-    {
-        std::lock_guard<std::mutex> lock(g_err_mu);
-        if (device >= 0 && device < kMaxDevices) p = g_err_ptr[device];
-    }
-    if (!p) return TIR_OK;
-    cudaError_t e = cudaMemcpy(bits, p, sizeof(uint32_t), cudaMemcpyDeviceToHost);
-    if (e == cudaSuccess && *bits) e = cudaMemset(p, 0, sizeof(uint32_t));
+    std::lock_guard<std::mutex> lock(g_err_mu);  // held until the taken bits are read
+    if (device < 0 || device >= kMaxDevices || !g_err_ptr[device]) return TIR_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e = launch_kernel(take_error_kernel, dim3(1), dim3(1), 0, st, false);
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(bits, g_paged_taken, sizeof(uint32_t), 0, cudaMemcpyDeviceToHost, st);
+    const cudaError_t done = cudaStreamSynchronize(st);
+    if (e == cudaSuccess) e = done;
     return e == cudaSuccess ? TIR_OK : paged_fail(e, "paged cache error word");
 }
 

@@ -1,6 +1,6 @@
 """What the paged cache operators promise, where it is easiest to break: quotients at the edge
 of a half step, weights far below a row's largest, pages outside the pool, infinities inside
-a row.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
+a row, reports of several streams.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
 import math
 
 import numpy as np
@@ -246,3 +246,41 @@ def test_nan_and_infinity_inside_a_row(cuda, tirlib, act, kind, max_len):
     tirlib.paged_attention(q, kv, lens, out, max_len=max_len)
     assert not torch.isfinite(out[0, :2]).any() and torch.equal(out[1], clean[1]) and torch.equal(out[0, 2:], clean[0, 2:])
     tirlib.ops_check()
+
+
+def test_reports_of_another_stream_are_not_lost(cuda, tirlib):
+    """A bad page, some work, then a bad length on one stream while another is being checked:
+    both are reported, wherever the second falls in a check of the first."""
+    torch = cuda
+    kv, _, _ = cache(torch, tirlib, "f32", 1, 64, 1, 64, 16, seed=13)
+    q = torch.randn(1, 4, 64, device="cuda")
+    out, x = torch.empty_like(q), torch.zeros(200000, device="cuda")
+    bad = tirlib.KVPages(kv.k, kv.v, torch.full_like(kv.table, -1))
+    one, long = (torch.tensor([n], dtype=torch.int32, device="cuda") for n in (1, 65))
+    busy, checked = torch.cuda.Stream(), torch.cuda.Stream()
+    tirlib.paged_attention(q, kv, one, out)
+    tirlib.ops_check()
+    lost = 0
+    for work in range(0, 80, 4):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            tirlib.paged_attention(q, bad, one, out)
+            for _ in range(work):
+                x.add_(1)
+            tirlib.paged_attention(q, kv, long, out)
+        for _ in range(20):
+            with torch.cuda.stream(busy):
+                graph.replay()
+            told, last = "", False
+            while True:
+                done = busy.query()
+                try:
+                    tirlib.ops_check(checked)
+                except tirlib.TirError as e:
+                    assert e.name == "INVALID_ARG"
+                    told += e.message
+                if last:
+                    break
+                last = done  # one more check after all is done
+            lost += "page id" not in told or "length" not in told
+    assert lost == 0
