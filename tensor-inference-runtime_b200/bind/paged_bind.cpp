@@ -326,4 +326,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_bind", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__paged_bind() { return PyModule_Create(&module); }
+// built_for: the torch whose headers this was compiled with
+PyMODINIT_FUNC PyInit__paged_bind() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", TIR_BIND_TORCH) < 0) Py_CLEAR(m);
+    return m;
+}

@@ -6,6 +6,7 @@ the library loads on a machine without a GPU.
 """
 import concurrent.futures
 import glob
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -20,7 +21,8 @@ INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG_DIR, "libtir.so")
 BIND_SRC = os.path.join(ROOT, "bind", "paged_bind.cpp")
-BIND = os.path.join(PKG_DIR, "_paged_bind.so")
+BIND = os.path.join(PKG_DIR, "_paged_bind" + sysconfig.get_config_var("EXT_SUFFIX"))
+BIND_STAMP = os.path.join(BUILD, "paged_bind.stamp")  # what BIND was compiled against
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2,-ffp-contract=off",
@@ -65,41 +67,63 @@ def _compile(src, verbose):
     return obj
 
 
-def build_bind():
-    """Compiles the torch binding of the paged cache operators (needs torch's
-    headers; without torch installed there are no tensors to bind)."""
-    if not _stale(BIND, [BIND_SRC, *_headers(), __file__]):
-        return BIND
-    spec = importlib.util.find_spec("torch")
-    if spec is None:
+def _bind_target():
+    """The torch and Python a binding is good for; None without torch."""
+    if importlib.util.find_spec("torch") is None:
         return None
-    torch_dir = os.path.dirname(spec.origin)
+    return f"torch {importlib.metadata.version('torch')}, {sysconfig.get_config_var('SOABI')}"
+
+
+def build_bind():
+    """Compiles the torch binding of the paged cache operators (needs torch's and
+    Python's headers; without torch installed there are no tensors to bind)."""
+    target = _bind_target()
+    if target is None:
+        return None
+    if not _stale(BIND, [BIND_SRC, *_headers(), __file__]) and os.path.exists(BIND_STAMP):
+        with open(BIND_STAMP) as f:
+            if f.read() == target:
+                return BIND
+    os.makedirs(BUILD, exist_ok=True)
+    import torch
+    torch_dir = os.path.dirname(torch.__file__)
     inc = os.path.join(torch_dir, "include")
     lib = os.path.join(torch_dir, "lib")
+    abi = int(getattr(torch._C, "_GLIBCXX_USE_CXX11_ABI", True))
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-w",
-           "-D_GLIBCXX_USE_CXX11_ABI=1", "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
-           "-I" + sysconfig.get_paths()["include"], BIND_SRC, "-o", BIND, "-L" + lib, "-Wl,-rpath," + lib,
-           "-ltorch_python", "-ltorch_cpu", "-lc10"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f'-DTIR_BIND_TORCH="{torch.__version__}"', "-I" + inc,
+           "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], BIND_SRC,
+           "-o", BIND, "-L" + lib, "-Wl,-rpath," + lib, "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{e}") from e
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    with open(BIND_STAMP, "w") as f:
+        f.write(target)
     return BIND
 
 
 def build(verbose=False):
-    """Compiles every CUDA/C++ source and links libtir.so (and, with torch
-    installed, its binding of the paged cache operators); returns its path."""
+    """Compiles every CUDA/C++ source and links libtir.so; returns its path.  With
+    torch installed its binding of the paged cache operators is compiled, too;
+    nothing else needs that, so a failure there is only printed (build_bind()
+    raises it, and the first call of such an operator says that it is missing)."""
     os.makedirs(BUILD, exist_ok=True)
     srcs = _sources()
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs)) + 1) as ex:
         bind = ex.submit(build_bind)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
-        bind.result()
-    if _stale(LIB, objs):
-        cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", LIB, *objs, "-lpthread", "-ldl", "-lrt"]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+        if _stale(LIB, objs):
+            cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", LIB, *objs, "-lpthread", "-ldl", "-lrt"]
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            if r.returncode != 0:
+                raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+        try:
+            bind.result()
+        except Exception as e:
+            print(f"{LIB} is built, the torch binding of the paged cache operators is not: {e}", file=sys.stderr)
     return LIB
 
 
