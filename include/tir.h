@@ -505,7 +505,9 @@ tir_status tir_kv_gather(const tir_kv_pages *kv, void *k_out, int64_t k_out_stri
  * the longest length (0: what the table holds), only sizes the split of long
  * rows over the GPU.  workspace: tir_paged_attention_workspace bytes (0: none
  * is needed, -1: sizes that are refused), 16-byte aligned, of any content, not
- * shared by calls that can run at the same time. */
+ * shared by calls that can run at the same time.  The bytes for some rows,
+ * max_len and window are enough for every call with no more rows, no longer
+ * max_len (0 is the longest) and no wider window (0 is the widest). */
 int64_t tir_paged_attention_workspace(const tir_kv_pages *kv, int64_t rows, int32_t q_heads, int64_t max_len,
                                       int64_t window);
 tir_status tir_paged_attention(const void *q, int64_t q_stride, const tir_kv_pages *kv, const int32_t *seq_lens,

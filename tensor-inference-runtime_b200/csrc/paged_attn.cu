@@ -98,10 +98,40 @@ int multiprocessors() {
 }
 
 struct Plan {
-    int nt, head_tiles;
+    int nt, head_tiles, sms;
     AttnShape shape;
+    int64_t units, slots;  // of the longest row; CTAs the GPU holds
     int32_t splits, min_units;
 };
+
+// What the sizes alone give.
+tir_status make_shape(const PagesView& kv, Elem cache, bool f32q, int64_t rows, int32_t q_heads, int64_t max_len,
+                      int64_t window, Plan* p) {
+    const int group = q_heads / kv.kv_heads;
+    p->nt = group <= 8 ? 1 : 2;
+    p->head_tiles = (group + 8 * p->nt - 1) / (8 * p->nt);
+    attn(nullptr, kv, cache, f32q, p->nt, rows, nullptr, &p->shape);
+    p->sms = multiprocessors();
+    if (p->sms <= 0) return fail(TIR_ERR_CUDA, "tir_paged_attention: no multiprocessor count for the current device");
+    int64_t n = static_cast<int64_t>(kv.max_pages) * kv.page_size;
+    if (max_len > 0) n = std::min(n, max_len);
+    if (window > 0) n = std::min(n, window);
+    p->units = (n + p->shape.unit - 1) / p->shape.unit;
+    p->slots = static_cast<int64_t>(p->sms) * p->shape.per_sm;
+    return TIR_OK;
+}
+
+// Parts beyond the first that a call may be divided into, in CTAs the GPU holds.
+constexpr int64_t kMostParts = 8;
+
+// Bytes that hold the parts of any call of these sizes or smaller ones.  The count of parts
+// that suits a call best goes up and down with its rows, so this takes what make_plan
+// looks at: rows * heads * (s - 1) <= kMostParts * slots, s <= units.
+int64_t workspace_of(const Plan& p, const PagesView& kv, int64_t rows, int32_t q_heads) {
+    if (p.units <= 1) return 0;
+    const int64_t most = kMostParts * p.slots / (kv.kv_heads * p.head_tiles), r = std::min(rows, most);
+    return std::min(most + r, r * p.units) * q_heads * (kv.dim + 2) * 4;
+}
 
 // How many CTAs share a row's head (s).  The time of a call is estimated twice,
 // for rows that are all of the longest length (waves of a start and a part's units)
@@ -132,18 +162,11 @@ SplitTime split_time(int64_t items, int64_t units, int64_t s, int64_t slots, flo
 
 tir_status make_plan(const PagesView& kv, Elem cache, bool f32q, int64_t rows, int32_t q_heads, int64_t max_len,
                      int64_t window, Plan* p) {
-    const int group = q_heads / kv.kv_heads;
-    p->nt = group <= 8 ? 1 : 2;
-    p->head_tiles = (group + 8 * p->nt - 1) / (8 * p->nt);
-    attn(nullptr, kv, cache, f32q, p->nt, rows, nullptr, &p->shape);
-    const int sms = multiprocessors();
-    if (sms <= 0) return fail(TIR_ERR_CUDA, "tir_paged_attention: no multiprocessor count for the current device");
-    int64_t n = static_cast<int64_t>(kv.max_pages) * kv.page_size;
-    if (max_len > 0) n = std::min(n, max_len);
-    if (window > 0) n = std::min(n, window);
-    const int64_t units = (n + p->shape.unit - 1) / p->shape.unit;
+    const tir_status rc = make_shape(kv, cache, f32q, rows, q_heads, max_len, window, p);
+    if (rc != TIR_OK) return rc;
+    const int sms = p->sms;
+    const int64_t units = p->units, slots = p->slots;
     const int64_t items = std::max<int64_t>(rows * kv.kv_heads * p->head_tiles, 1);
-    const int64_t slots = static_cast<int64_t>(sms) * p->shape.per_sm;
     const float unit_sm = static_cast<float>(p->shape.unit * kv.dim * 2 * p->shape.bytes * sms / kBytesPerUs);
     int64_t tries[48];
     SplitTime times[48];
@@ -159,7 +182,7 @@ tir_status make_plan(const PagesView& kv, Elem cache, bool f32q, int64_t rows, i
     };
     for (int64_t w = 1; w <= 3; ++w)  // parts that fill whole waves
         if (const int64_t s = w * slots / items; s > 1 && s <= units) consider(s);
-    for (int64_t s = 1; s <= units && (s - 1) * items <= 8 * slots; s += 1 + s / 6) consider(s);
+    for (int64_t s = 1; s <= units && (s - 1) * items <= kMostParts * slots; s += 1 + s / 6) consider(s);
     int64_t best = 1;
     float least = 1e30f;
     for (int i = 0; i < n_tries; ++i) {
@@ -174,10 +197,6 @@ tir_status make_plan(const PagesView& kv, Elem cache, bool f32q, int64_t rows, i
     // shorter rows get fewer parts, down to half the length of the longest row's
     p->min_units = static_cast<int32_t>(std::max<int64_t>((units + best - 1) / best / 2, 1));
     return TIR_OK;
-}
-
-int64_t workspace_of(const Plan& p, int64_t rows, int32_t q_heads, int32_t dim) {
-    return p.splits > 1 ? rows * q_heads * p.splits * (dim + 2) * 4 : 0;
 }
 
 }  // namespace
@@ -209,8 +228,8 @@ int64_t tir_paged_attention_workspace(const tir_kv_pages* kv, int64_t rows, int3
     int64_t most = 0;
     for (const bool f32q : {false, true}) {
         Plan p;
-        if (make_plan(view, cache, f32q, rows, q_heads, max_len, window, &p) != TIR_OK) return -1;
-        most = std::max(most, workspace_of(p, rows, q_heads, kv->dim));
+        if (make_shape(view, cache, f32q, rows, q_heads, max_len, window, &p) != TIR_OK) return -1;
+        most = std::max(most, workspace_of(p, view, rows, q_heads));
     }
     return most;
 }
@@ -239,7 +258,7 @@ tir_status tir_paged_attention(const void* q, int64_t q_stride, const tir_kv_pag
     Plan p;
     rc = make_plan(view, cache, act == Elem::F32, rows, q_heads, max_len, window, &p);
     if (rc != TIR_OK) return rc;
-    const int64_t need = workspace_of(p, rows, q_heads, kv->dim);
+    const int64_t need = p.splits > 1 ? workspace_of(p, view, rows, q_heads) : 0;
     if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
         return fail(TIR_ERR_INVALID_ARG, std::string(who) + ": needs a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
     AttnArgs a{};

@@ -944,7 +944,7 @@ def kv_gather(kv, k_out, v_out, seqs, positions, stream=None):
 
 
 def paged_attention_workspace(kv, rows, q_heads, max_len=0, window=0):
-    """Bytes of workspace paged_attention needs for these sizes (0: none)."""
+    """Bytes of workspace paged_attention needs for these sizes or smaller ones (0: none)."""
     return _bind().workspace(kv.ref, rows, q_heads, max_len, window)
 
 

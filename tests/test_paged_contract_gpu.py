@@ -1,6 +1,7 @@
 """What the paged cache operators promise, where it is easiest to break: quotients at the edge
 of a half step, weights far below a row's largest, pages outside the pool, infinities inside
-a row, reports of several streams.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
+a row, reports of several streams,
+workspaces sized once.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
 import math
 
 import numpy as np
@@ -284,3 +285,29 @@ def test_reports_of_another_stream_are_not_lost(cuda, tirlib):
                 last = done  # one more check after all is done
             lost += "page id" not in told or "length" not in told
     assert lost == 0
+
+
+@pytest.mark.parametrize("kind,q_heads,kv_heads,dim", [("bf16", 32, 8, 128), ("f32", 32, 4, 64), ("q8_0", 8, 1, 256), ("f16", 71, 1, 64)])
+def test_workspace_of_the_largest_sizes_serves_smaller_ones(cuda, tirlib, kind, q_heads, kv_heads, dim):
+    """The bytes needed never shrink with more rows, a longer max_len or a wider window."""
+    torch = cuda
+    rows, ctx = 300, 8192
+    t = dtype(torch, kind)
+    pool = torch.zeros(2, 4, 16, kv_heads, dim, dtype=t, device="cuda")
+    scale = torch.ones(2, 4, 16, kv_heads, dim // 32, dtype=torch.float16, device="cuda") if kind == "q8_0" else (None, None)
+    kv = tirlib.KVPages(pool[0], pool[1], torch.zeros(rows, ctx // 16, dtype=torch.int32, device="cuda"), scale[0], scale[1])
+    act = torch.float32 if kind in ("f32", "q8_0") else t
+    q = torch.zeros(rows, q_heads, dim, dtype=act, device="cuda")
+    out = torch.empty_like(q)
+    lens = torch.full((rows,), 100, dtype=torch.int32, device="cuda")
+    ws = torch.empty(tirlib.paged_attention_workspace(kv, rows, q_heads, ctx), dtype=torch.uint8, device="cuda")
+    sizes = lambda n, m, w: tirlib.paged_attention_workspace(kv, n, q_heads, m, w)
+    for a, b in zip((1, 2, 3, 7, 20, 64, 100, 150, 200, 256), (2, 3, 7, 20, 64, 100, 150, 200, 256, 300)):
+        for m in (1, 100, 2048, ctx):
+            assert sizes(a, m, 0) <= sizes(b, m, 0)
+            assert sizes(a, m, 0) <= sizes(a, ctx, 0) <= ws.numel()
+            assert sizes(a, ctx, m) <= sizes(a, ctx, 0)
+        for m in (1, 2048, ctx):
+            tirlib.paged_attention(q[:a], kv, lens, out[:a], max_len=m, workspace=ws)
+    torch.cuda.synchronize()
+    tirlib.ops_check()
