@@ -311,3 +311,40 @@ def test_workspace_of_the_largest_sizes_serves_smaller_ones(cuda, tirlib, kind, 
             tirlib.paged_attention(q[:a], kv, lens, out[:a], max_len=m, workspace=ws)
     torch.cuda.synchronize()
     tirlib.ops_check()
+
+
+@pytest.mark.parametrize("act,kind,dim", [("f32", "f32", 64), ("bf16", "bf16", 128), ("f32", "q8_0", 64)])
+def test_divided_rows_agree_whatever_max_len_says(cuda, tirlib, act, kind, dim):
+    """The number of parts changes an output by no more than the two roundings' bounds, and
+    the same call gives the same bits; max_len does divide the rows."""
+    torch = cuda
+    lens = [9001, 1, 0, 4097]
+    kv, values, _ = cache(torch, tirlib, kind, 4, 9001, 1, dim, 16, seed=14)
+    q = torch.randn(4, 5, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(15)).to(dtype(torch, act))
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    assert tirlib.paged_attention_workspace(kv, 4, 5) > 0 and tirlib.paged_attention_workspace(kv, 4, 5, 9001) > 0
+    assert tirlib.paged_attention_workspace(kv, 4, 5, 1) == 0
+    outs = []
+    for max_len in (0, 9001, 1, 3000):
+        pair = torch.empty(2, *q.shape, dtype=q.dtype, device="cuda")
+        for o in pair:
+            tirlib.paged_attention(q, kv, n, o, max_len=max_len)
+        assert torch.equal(pair[0], pair[1])
+        outs.append(pair[0].double())
+    ref, mass, big = attention_ref(torch, q, values(), lens, 1 / math.sqrt(dim), 0)
+    ut = torch.finfo(q.dtype).eps / 2
+    e = (2 * dim / 8 + 4) * 2.0 ** -23 * big + 2.0 ** -20
+    bound = 2 * ((2 * e + 9001 / 8 * 2.0 ** -23 + 2.0 ** -20) * mass + ut * ref.abs() + 2.0 ** -25)
+    for o in outs[1:]:
+        assert ((o - outs[0]).abs() <= bound).all()
+
+
+def test_too_small_a_workspace_is_refused(cuda, tirlib):
+    torch = cuda
+    kv, _, _ = cache(torch, tirlib, "f32", 1, 20000, 1, 64, 16)
+    need = tirlib.paged_attention_workspace(kv, 1, 4)
+    assert need > 0
+    q, lens = torch.zeros(1, 4, 64, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(tirlib.TirError) as e:
+        tirlib.paged_attention(q, kv, lens, torch.empty_like(q), workspace=torch.empty(need - 1, dtype=torch.uint8, device="cuda"))
+    assert e.value.name == "INVALID_ARG" and "workspace" in e.value.message
