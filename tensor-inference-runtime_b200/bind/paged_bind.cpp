@@ -252,15 +252,13 @@ void paged_attention(PyObject* const* a) {
         if (w.get_device() != dev || !w.is_contiguous()) bad("workspace must be a contiguous tensor on device " + std::to_string(dev));
         ws = w.data_ptr();
         bytes = static_cast<int64_t>(w.nbytes());
-    } else {
+    } else if (a[9] == Py_None || reinterpret_cast<int64_t>(st) == current_stream(dev)) {
         bytes = S.workspace(kv, x.n, static_cast<int32_t>(qh), max_len, window);
         if (bytes > 0) {
-            if (a[9] != Py_None && reinterpret_cast<int64_t>(st) != current_stream(dev))
-                bad("paged_attention on another stream than the current one needs a workspace");
             own = at::empty({bytes}, q.options().dtype(at::kByte));
             ws = own.data_ptr();
         }
-    }
+    }  // on another stream a call that divides its rows is refused: the allocator would not know of its work
     check(S.paged_attention(x.p, x.stride, kv, lens, o.p, o.stride, x.n, static_cast<int32_t>(qh), code,
                             static_cast<float>(number(a[5])), max_len, window, ws, bytes, st));
 }

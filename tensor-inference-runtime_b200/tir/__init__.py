@@ -953,5 +953,5 @@ def paged_attention(q, kv, seq_lens, out, scale=0.0, max_len=0, window=0, worksp
     over the last `window` (0: all) of the seq_lens[r] positions of table row r;
     zeros for a row of length 0.  workspace: a uint8 tensor of
     paged_attention_workspace bytes; without one it is taken from torch's allocator
-    for the call, on the current stream."""
+    for the call on the current stream; on another one a call that needs it is refused."""
     _bind().paged_attention(q, kv.ref, kv.device, seq_lens, out, scale, max_len, window, workspace, _raw(stream))

@@ -348,3 +348,26 @@ def test_too_small_a_workspace_is_refused(cuda, tirlib):
     with pytest.raises(tirlib.TirError) as e:
         tirlib.paged_attention(q, kv, lens, torch.empty_like(q), workspace=torch.empty(need - 1, dtype=torch.uint8, device="cuda"))
     assert e.value.name == "INVALID_ARG" and "workspace" in e.value.message
+
+
+def test_another_stream_without_a_workspace(cuda, tirlib):
+    """Rows that are not divided need none; a call that would divide them is refused there,
+    and takes its workspace from torch on the current stream."""
+    torch = cuda
+    kv, values, _ = cache(torch, tirlib, "f32", 64, 256, 4, 64, 16, seed=16)
+    q = torch.randn(64, 32, 64, device="cuda")
+    lens = torch.full((64,), 256, dtype=torch.int32, device="cuda")
+    out, other = torch.empty_like(q), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    tirlib.paged_attention(q, kv, lens, out, max_len=256, stream=other)
+    torch.cuda.synchronize()
+    check_attention(torch, out, *attention_ref(torch, q, values(), [256] * 64, 0.125, 0), 64, 256)
+    kv, values, _ = cache(torch, tirlib, "f32", 1, 20000, 1, 64, 16, seed=17)
+    q, lens = q[:1, :4], lens[:1] * 70
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    with pytest.raises(tirlib.TirError) as e:
+        tirlib.paged_attention(q, kv, lens, out, stream=other)
+    assert e.value.name == "INVALID_ARG" and "workspace" in e.value.message
+    tirlib.paged_attention(q, kv, lens, out, stream=torch.cuda.current_stream())
+    check_attention(torch, out, *attention_ref(torch, q, values(), [17920], 0.125, 0), 64, 17920)
