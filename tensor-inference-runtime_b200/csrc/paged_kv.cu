@@ -35,7 +35,7 @@ constexpr uint32_t FULL = 0xffffffffu;
 constexpr int kRowThreads = 128;
 constexpr int kMaxDevices = 64;
 
-std::mutex g_err_mu;
+std::mutex g_err_mu, g_take_mu;
 uint32_t* g_err_ptr[kMaxDevices];
 
 struct RowArgs {
@@ -612,8 +612,11 @@ tir_status paged_error_word(uint32_t** out) {
 
 tir_status paged_take_error(int device, void* stream, uint32_t* bits) {
     *bits = 0u;
-    std::lock_guard<std::mutex> lock(g_err_mu);  // held until the taken bits are read
-    if (device < 0 || device >= kMaxDevices || !g_err_ptr[device]) return TIR_OK;
+    {
+        std::lock_guard<std::mutex> lock(g_err_mu);  // not over the wait: launches take it, too
+        if (device < 0 || device >= kMaxDevices || !g_err_ptr[device]) return TIR_OK;
+    }
+    std::lock_guard<std::mutex> lock(g_take_mu);  // until the taken bits are read
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = launch_kernel(take_error_kernel, dim3(1), dim3(1), 0, st, false);
     if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(bits, g_paged_taken, sizeof(uint32_t), 0, cudaMemcpyDeviceToHost, st);

@@ -3,6 +3,7 @@ of a half step, weights far below a row's largest, pages outside the pool, infin
 a row, reports of several streams,
 workspaces sized once.  Tolerances as in test_paged_gpu.py, whose helpers these tests use."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -285,6 +286,42 @@ def test_reports_of_another_stream_are_not_lost(cuda, tirlib):
                 last = done  # one more check after all is done
             lost += "page id" not in told or "length" not in told
     assert lost == 0
+
+
+def test_checks_and_calls_from_several_threads(cuda, tirlib):
+    """Two threads check streams of their own while a third calls operators on both, a bad
+    page among them now and then: all come to an end, and the bad pages are reported."""
+    torch = cuda
+    kv, _, _ = cache(torch, tirlib, "f32", 2, 64, 1, 64, 16, seed=18)
+    bad = tirlib.KVPages(kv.k, kv.v, torch.full_like(kv.table, -1))
+    q, lens = torch.randn(2, 4, 64, device="cuda"), torch.tensor([64, 3], dtype=torch.int32, device="cuda")
+    outs = torch.empty(2, *q.shape, device="cuda")
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    told, failed, done = [], [], threading.Event()
+
+    def check(stream):
+        while True:
+            last = done.is_set()
+            try:
+                tirlib.ops_check(stream)
+            except tirlib.TirError as e:
+                (told if e.name == "INVALID_ARG" and "page id" in e.message else failed).append(str(e))
+            if last:
+                return
+
+    threads = [threading.Thread(target=check, args=(s,)) for s in streams]
+    for t in threads:
+        t.start()
+    for i in range(400):
+        for s, out in zip(streams, outs):
+            tirlib.paged_attention(q, bad if i % 50 == 7 else kv, lens, out, stream=s)
+    torch.cuda.synchronize()
+    done.set()
+    for t in threads:
+        t.join(timeout=60)
+        assert not t.is_alive()
+    assert told and not failed
 
 
 @pytest.mark.parametrize("kind,q_heads,kv_heads,dim", [("bf16", 32, 8, 128), ("f32", 32, 4, 64), ("q8_0", 8, 1, 256), ("f16", 71, 1, 64)])
