@@ -500,7 +500,8 @@ tir_status tir_kv_gather(const tir_kv_pages *kv, void *k_out, int64_t k_out_stri
  * output non-finite, a NaN or infinity in a value its element of the output
  * (Q8_0: its block of 32); a key with an infinity whose score is -inf has no
  * weight, as in the formula, or makes the head non-finite, and a row of nothing
- * else is non-finite.  Several query tokens of one sequence are rows of their own, with
+ * else is non-finite (f32 values within 2^-8 of the type's largest may count as
+ * infinite).  Several query tokens of one sequence are rows of their own, with
  * the same pages in the table and lengths that end at each.  max_len, at least
  * the longest length (0: what the table holds), only sizes the split of long
  * rows over the GPU.  workspace: tir_paged_attention_workspace bytes (0: none

@@ -138,10 +138,10 @@ int64_t workspace_of(const Plan& p, const PagesView& kv, int64_t rows, int32_t q
 // and for rows spread evenly below it (all units over the GPU, starts, half a
 // longest part), and the s with the least sum of the two, each over its least, is
 // taken: the lengths are on the device, and a count that suits both costs either
-// little.  Measured on B200: 64 rows x 4 heads x 2048 positions in f32 take 50 us with
-// s = 1, 56 with 3, 60 with 4; 64 rows x 8 heads up to 8192 in bf16 194 with 1, 173 with 4,
-// 189 with 12; one row of 16000 beside 63 of 300 172 with 1, 41 with 6; one row of
-// 131071 1324 with 1, 91 with 37.
+// little.  Measured on B200, the choice first: 64 rows x 4 heads x 2048 positions in f32
+// take 49 us with s = 1, 56 with 3, 62 with 4; 64 rows x 8 heads up to 8192 in bf16 174 with
+// 4, 198 with 1, 190 with 12; one row of 16000 beside 63 of 300 45 with 5, 176 with 1, 40 with
+// 6; one row of 131071 87 with 18, 1303 with 1, 94 with 37.
 constexpr float kStart = 2.0f, kJoin = 2.3f, kJoinRow = 1.0f / 1200.0f;  // us
 constexpr float kBytesPerUs = 6.2e6f;
 

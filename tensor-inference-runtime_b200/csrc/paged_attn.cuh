@@ -9,9 +9,12 @@
 // or 32 positions in turn, each with a ring of cp.async half tiles (keys, values,
 // keys, ...) and a softmax (m, l, o) of its own, so the loop has no CTA barrier.
 // The warps' parts meet in shared memory, those of different CTAs in
-// paged_attn_join.  64 rows of 2048 positions take 86 us in bf16 with 8 heads of 128
-// (6.2 TB/s), 50 in f32 with 4 heads of 64 (5.4 TB/s: every value in two tf32 parts)
-// and 24.5 in Q8_0 (2.9 TB/s: bound by the instructions that convert).
+// paged_attn_join.  64 rows of 2048 positions take 84 to 87 us in bf16 with 8 heads of
+// 128 (6.3 TB/s: bound by memory), 49.5 in f32 with 4 heads of 64 (5.4 TB/s) and 24 in
+// Q8_0 (3.0 TB/s).  The last two are bound by latency: 256 CTAs leave a scheduler 1.7
+// warps, each of which issues every 3.4 to 3.8 cycles (most of them the fixed latency of
+// the instruction before: two tf32 parts of every value, the conversions of every quant),
+// so that a scheduler issues in half of its cycles and no pipe is busy for above 46 %.
 //
 // Products on the tensor cores (mma.sync: with 8 query heads a tile is M = 16
 // positions or dimensions by N = 8 heads, far below the smallest tcgen05 tile,
@@ -241,9 +244,9 @@ struct AttnCfg {
     static constexpr int UNIT = WARPS * TILE;
     static constexpr int FIXED = QBYTES + HEADS * 4 + WARPS * HEADS * 8;
     // a warp's ring: SLOTS half tiles (keys, values, keys, ...), an odd number, so that
-    // a step on keys asks for keys.  Three CTAs an SM for heads of 64 (64 x 256 in f32:
-    // 12.5 us, 13.2 with two), two for wider ones where three slots fit (64 x 2048 in
-    // bf16 with heads of 128: 87 us, 95 with three).
+    // a step on keys asks for keys.  Three CTAs an SM for heads of 64 (64 x 2048 in f32:
+    // 49.5 us, 51.1 with two; 64 x 256 10.3 and 10.6), two for wider ones where three slots
+    // fit (64 x 2048 in bf16 with heads of 128: 86 us, 98 with three).
     static constexpr int fits(int ctas) { return (227 * 1024 / ctas - 1024 - FIXED) / (WARPS * HALF); }
     static constexpr int PER_SM = fits(3) >= 3 && D == 64 && NT == 1 ? 3 : fits(2) >= 3 ? 2 : 1;
     static constexpr int SLOTS = fits(PER_SM) >= 7 ? 7 : fits(PER_SM) >= 5 ? 5 : 3;
@@ -934,10 +937,10 @@ cudaError_t launch_attn_as(const AttnArgs& a, const PagesView& kv, int64_t rows,
 
 // What the split's estimate knows of the kernel that a cache type, head size and
 // query type get: CTAs an SM holds, the positions of a unit, the bytes an element
-// weighs in an SM that holds several (Q8_0: half as much again, its conversions are
-// the bound there), and the time of a unit in a CTA that has an SM to itself
-// (measured on B200: f32 0.93 us with heads of 64 and 1.6 with 128, 16-bit types 0.65
-// with 128 and 1.05 with 256, Q8_0 0.88 with 64 and 1.3 with 128).
+// weighs in an SM that holds several (Q8_0: half as much again, its
+// instructions take longer than its bytes), and the time of a unit in a CTA that has an SM to itself
+// (measured on B200: f32 0.95 us with heads of 64 and 1.5 with 128, 16-bit types 0.60
+// with 128 and 0.83 with 256, Q8_0 0.88 with 64 and 1.27 with 128).
 struct AttnShape {
     int per_sm, unit;
     float bytes, lone;

@@ -120,7 +120,7 @@ __device__ __forceinline__ float rsqrt_approx(float x) {
 //   where |x| / |d| >= h - half of f32's step below h, and |x| - h |d| is exact in
 //   one fma (x and h d agree in their leading 13 bits, h d has eight more than d).
 //   Values of 16 bits meet such halves often: x = max / 2 gives 63.5 (dividing there
-//   took 21.4 us for 8192 x 16 heads of 128 in bf16, this took 18.1);
+//   takes 20.3 us for 8192 x 16 heads of 128 in bf16, this 16.9);
 // * steps too small or too large for either, and NaN, are divided by.
 __device__ __forceinline__ void quantise8(const float* f, int lane4, uint2* quants, float* step) {
     float hi = max3_nan(max3_nan(f[0], f[1], f[2]), max3_nan(f[3], f[4], f[5]), max_nan(f[6], f[7]));
@@ -193,10 +193,10 @@ __device__ __forceinline__ bool find_slot(const RowArgs& a, const PagesView& kv,
 enum class Mode { Rows, Fused, FusedQ8, Append, AppendQ8 };
 
 // Blocks an SM holds: eight of 64 registers a thread where a lane's four heads fit
-// them (4109 tokens of 48 heads of 128 in f16: 22.7 us, with six 23.5; 8 x 1024 tokens
-// of 16 heads of 128 in bf16 to Q8_0 and back: 25.3 and 26.0); where they would spill,
+// them (4109 tokens of 48 heads of 128 in f16: 20.8 us, with six 22.0; 8 x 1024 tokens
+// of 16 heads of 128 in bf16 to Q8_0 and back: 25.2 and 25.8); where they would spill,
 // six of 80 (norm and rotation of halves only, 8192 tokens of 40 heads of 128 in bf16:
-// 33.9 us, with eight 35.3).
+// 32.1 us, with eight 37.4; into Q8_0, 48 heads: 52.7 and 55.3).
 template <Elem A, Mode M, int HPG, bool H>
 constexpr int kMinBlocks = HPG == 4 && (A == Elem::F32 || M == Mode::FusedQ8 || (M == Mode::Rows && H)) ? 6 : 8;
 
@@ -208,11 +208,12 @@ constexpr int kMinBlocks = HPG == 4 && (A == Elem::F32 || M == Mode::FusedQ8 || 
 // a launch does and H that halves are paired in the rotation, so that each keeps
 // only the registers it needs (more warps: the kernel is bound by issue and memory
 // alike).  With paired halves a lane of the rotated part holds four elements of
-// either half, so that it turns pairs of its own with half the angles (with eight
-// consecutive ones and the partners by shuffles 4109 tokens of 48 heads of 128 in
-// f16 took 25.9 us, 64 in bf16 3.0; this takes 20.8 and 2.3); a block to be
-// quantised then goes back to consecutive lanes by as many shuffles.  8192 tokens of
-// 36 heads of 64 in f32 take 24.4 us (6.2 TB/s), the 4109 in f16 run at 4.9 TB/s.
+// either half, so that it turns pairs of its own with half the angles (instead of eight
+// consecutive ones and the partners by shuffles; together with the packed arithmetic and
+// the grid by head and token that took 4109 tokens of 48 heads of 128 in f16 from 25.9 to
+// 21.3 us, 64 in bf16 from 3.0 to 2.5); a block to be quantised then goes back to
+// consecutive lanes by as many shuffles.  8192 tokens of 36 heads of 64 in f32 take 24.2 us
+// (6.2 TB/s), the 4109 in f16 20.8 (4.9 TB/s).
 template <Elem A, int D, Mode M, int HPG, bool H>
 __global__ void __launch_bounds__(kRowThreads, kMinBlocks<A, M, HPG, H>) rows_kernel(const RowArgs a, const PagesView kv, const Elem cache) {
     constexpr int G = D / 8;
@@ -421,8 +422,9 @@ cudaError_t by_type(Elem e, int32_t dim, F&& f) {
 
 // Heads a group of lanes takes, and the grid: four once one each would give every
 // SM two blocks or more for each of its four schedulers (8192 tokens of 36 heads of
-// 64 in f32: 31.6 us with one, 24.4 with four; 512 tokens of 48 heads of 128 in
-// bf16: 5.2 and 4.1, 256 3.4 and 3.5), one below that (64 tokens: 2.3 us).
+// 64 in f32: 27.4 us with one, 24.2 with four; with cache write 512 tokens of 48 heads of
+// 128 in bf16: 6.5 and 5.4, 256 3.7 both), one below that (64 tokens: 2.3 and 3.1 us;
+// read-back of 2047 positions of 4 heads of 64 in f32 2.6 and 2.9, of 65536 47.9 and 44.5).
 struct RowShape {
     bool four;
     dim3 grid;  // chunks of one kind of head, blocks of tokens
@@ -443,10 +445,10 @@ bool row_shape(RowArgs* a, int32_t dim, RowShape* s) {
 }
 
 // Both kernels and the attention are launched to take over as soon as the work before them
-// is over (64 tokens with cache write: 2.3 us instead of 2.5, called back to back 4 us
-// instead of 5), but none lets the next one in before its own end: blocks that start
-// while others still run gather on the SMs that come free first (64 tokens' write, then
-// attention over 64 x 2048 in Q8_0: 33.8 us so, 27.2 without).
+// is over (64 tokens with cache write: 2.3 us instead of 2.5; attention of one row of 144,
+// called back to back: 6.1 instead of 8.2), but none lets the next one in before its own
+// end: blocks that start while others still run gather on the SMs that come free first (64
+// tokens' write, then attention over 64 x 2048 in Q8_0: 33.8 us so, 27.0 without).
 template <Mode M>
 cudaError_t launch_mode(const RowArgs& a, const PagesView& kv, Elem act, Elem cache, int32_t dim, const RowShape& s, cudaStream_t stream) {
     return by_type(act, dim, [&](auto el, auto d) {
