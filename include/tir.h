@@ -504,7 +504,8 @@ tir_status tir_kv_gather(const tir_kv_pages *kv, void *k_out, int64_t k_out_stri
  * infinite).  Several query tokens of one sequence are rows of their own, with
  * the same pages in the table and lengths that end at each.  max_len, at least
  * the longest length (0: what the table holds), only sizes the split of long
- * rows over the GPU.  workspace: tir_paged_attention_workspace bytes (0: none
+ * rows over the GPU; far above the lengths it divides them less.
+ * workspace: tir_paged_attention_workspace bytes (0: none
  * is needed, -1: sizes that are refused), 16-byte aligned, of any content, not
  * shared by calls that can run at the same time.  The bytes for some rows,
  * max_len and window are enough for every call with no more rows, no longer
