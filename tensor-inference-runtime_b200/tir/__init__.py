@@ -835,8 +835,9 @@ def _bind():
             from . import _paged_bind as m
         except ImportError as e:
             raise ImportError(f"the torch binding of the paged cache operators cannot be loaded ({e}): {how}") from e
-        if m.built_for != torch.__version__:
-            raise ImportError(f"the torch binding of the paged cache operators is for torch {m.built_for}, "
+        built_for = getattr(m, "built_for", "of an earlier build")
+        if built_for != torch.__version__:
+            raise ImportError(f"the torch binding of the paged cache operators is for torch {built_for}, "
                               f"not {torch.__version__}: {how}")
         addresses = [C.cast(getattr(lib(), "tir_" + n), C.c_void_p).value
                      for n in ("last_error", "qk_norm_rope", "qk_norm_rope_append", "kv_append", "kv_gather",

@@ -43,10 +43,11 @@ def test_the_binding_is_compiled_again_for_another_torch_or_python(elsewhere, mo
         elsewhere.build_bind()
 
 
-@pytest.mark.parametrize("found", ["for another torch", "nothing"])
+@pytest.mark.parametrize("found", ["for another torch", "of an earlier build", "nothing"])
 def test_a_binding_that_does_not_fit_is_refused_on_first_use(tirlib, monkeypatch, found):
     torch = pytest.importorskip("torch")
-    module = None if found == "nothing" else types.SimpleNamespace(built_for="0.0")
+    module = {"for another torch": types.SimpleNamespace(built_for="0.0"), "of an earlier build": types.SimpleNamespace(),
+              "nothing": None}[found]
     monkeypatch.setattr(tirlib, "_bind_module", None)
     monkeypatch.setitem(sys.modules, "tir._paged_bind", module)
     if hasattr(tirlib, "_paged_bind"):
