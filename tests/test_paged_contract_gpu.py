@@ -387,6 +387,26 @@ def test_too_small_a_workspace_is_refused(cuda, tirlib):
     assert e.value.name == "INVALID_ARG" and "workspace" in e.value.message
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q_heads,kv_heads", [(9, 1), (17, 1), (24, 2), (71, 1)])
+@pytest.mark.parametrize("act,kind", [("f16", "f16"), ("f32", "f16"), ("bf16", "q8_0"), ("f32", "q8_0"), ("f32", "bf16")])
+def test_large_head_groups(cuda, tirlib, act, kind, q_heads, kv_heads, dim):
+    """More than eight query heads on a key-value head, in every type whose weights have parts
+    of their own place; short rows, one over many tiles, a window."""
+    torch = cuda
+    lens = [5, 100, 0, 1211]
+    kv, values, poison = cache(torch, tirlib, kind, 4, 1211, kv_heads, dim, 16, seed=q_heads)
+    q = torch.randn(4, q_heads, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(19)).to(dtype(torch, act))
+    vals = values()
+    poison(lens)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for window in (0, 333):
+        out = torch.empty_like(q)
+        tirlib.paged_attention(q, kv, n, out, window=window)
+        check_attention(torch, out, *attention_ref(torch, q, vals, lens, 1 / math.sqrt(dim), window), dim, 1211)
+    tirlib.ops_check()
+
+
 def test_another_stream_without_a_workspace(cuda, tirlib):
     """Rows that are not divided need none; a call that would divide them is refused there,
     and takes its workspace from torch on the current stream."""
